@@ -338,9 +338,8 @@ def _plain_block_case(s):
     at = offsets[:-1, None] + torch.arange(s["most"], device=a.device)
     real = torch.arange(s["most"], device=a.device) < counts[:, None]
     inner = _dequantize(*_quantize(_plain_product(a, s["w13"], s["s13"], at, real, True)))
-    gates = torch.where(slot_map >= 0, s["gate"].reshape(-1)[slot_map.clamp_min(0).long()], 0.0)
-    rows = (_plain_product(inner, s["w2"], s["s2"], at, real, False) * gates[:, None]).to(torch.bfloat16)
-    return {"out": _plain_unsort(rows, slots, None, None), "residual": h}
+    rows = _plain_product(inner, s["w2"], s["s2"], at, real, False).to(torch.bfloat16)
+    return {"out": _plain_unsort(rows, slots, s["gate"], None), "residual": h}
 
 
 # ----------------------------------------------------------------------------------------------- one pass
@@ -581,6 +580,6 @@ def exact(case, seed):
         token, k = (s["idx"] == e).nonzero(as_tuple=True)
         if len(token):
             q, scales = _exact_blocks(_exact_expert(rows[token], s["w13"][e], s["s13"][e], True))
-            part = _exact_expert(_exact_rows(q.to(E4M3), scales), s["w2"][e], s["s2"][e], False) * s["gate"][token, k].double()[:, None]
-            out.index_add_(0, token, part.to(torch.bfloat16).double())  # rows travel back in 16 bits
+            part = _exact_expert(_exact_rows(q.to(E4M3), scales), s["w2"][e], s["s2"][e], False).to(torch.bfloat16)  # rows travel back in 16 bits
+            out.index_add_(0, token, part.double() * s["gate"][token, k].double()[:, None])
     return {"out": out, "residual": total}
