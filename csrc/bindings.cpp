@@ -4,6 +4,7 @@
 
 #include "flag_queue.hpp"
 #include "gemm_api.hpp"
+#include "op_api.hpp"
 #include "pipeline.hpp"
 #include "unit_queue.hpp"
 
@@ -287,4 +288,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     });
 
     nep::bind_gemm(m);
+    nep::bind_ops(m);
 }

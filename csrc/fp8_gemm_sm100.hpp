@@ -1,0 +1,34 @@
+// Launch interface of the 8-bit grouped GEMM with a scale for each block of 128 (fp8_gemm_sm100.cu).
+#pragma once
+#include <cstdint>
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+namespace nep {
+namespace fp8 {
+
+constexpr int kMaxExperts = 1024;
+enum Fp8Status : uint32_t { kPipeTimeout = 101, kBadOffsets = 106 };
+
+struct Args {
+    const uint8_t* a;               // e4m3 [rows, k]
+    const uint8_t* w;               // e4m3 [experts, (2 *) n, k]
+    const float* a_scales;          // [rows, k_blocks]
+    const float* w_scales;          // [experts, (2 *) n_blocks, k_blocks]
+    const int64_t* expert_offsets;  // [experts + 1], or null: one expert owns all rows
+    const int64_t* expert_counts;   // [experts] rows that exist, or null: all rows of the range
+    const float* row_scale;         // or null: [rows]
+    __nv_bfloat16* out;             // [rows, n], or
+    uint8_t* q;                     // e4m3 [rows, n] with
+    float* scales;                  // [rows, n_blocks]
+    int64_t rows;
+    int experts, k, n;              // n: output columns (with SwiGLU half of the weight's rows)
+    int k_blocks, n_blocks;         // of 128
+    int swiglu;
+    uint32_t* status;               // 2 words: first error code, detail
+};
+cudaError_t launch(const Args& args, int sms, cudaStream_t stream);
+
+}  // namespace fp8
+}  // namespace nep

@@ -1,0 +1,396 @@
+// Python bindings of the operators around 8-bit experts: norm, token order, block-scaled product.  They check their arguments,
+// allocate what they return on the caller's stream and launch there; none of them waits for the device.
+#include "op_api.hpp"
+
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+
+#include "fp8_gemm_sm100.hpp"
+#include "peer_window.hpp"
+#include "rms_norm.hpp"
+#include "token_order.hpp"
+
+namespace nep {
+namespace {
+
+// Messages hold no numbers but through std::to_string: numeric operator<< on iostreams is avoided throughout this extension.
+static_assert(order::kMaxTopk == 32 && order::kMaxExperts == 1024 && fp8::kMaxExperts == 1024, "limits named in messages");
+
+using OptTensor = c10::optional<at::Tensor>;
+
+// Element types in the numbering that norm::Type and order::Type share.
+int row_type(const at::Tensor& t, const char* name) {
+    const auto s = t.scalar_type();
+    TORCH_CHECK(s == at::kBFloat16 || s == at::kHalf || s == at::kFloat, name, " must be bfloat16, float16 or float32");
+    return s == at::kBFloat16 ? 0 : s == at::kHalf ? 1 : 2;
+}
+
+void check_rows(const at::Tensor& t, const char* name) {
+    TORCH_CHECK(t.is_cuda() && t.dim() == 2 && t.is_contiguous(), name, " must be a contiguous two-dimensional CUDA tensor");
+}
+
+void check_like(const OptTensor& t, const at::Tensor& x, const char* name) {
+    if (!t.has_value()) return;
+    TORCH_CHECK(t->is_cuda() && t->device() == x.device() && t->scalar_type() == x.scalar_type() && t->sizes() == x.sizes() && t->is_contiguous(), name,
+                " must be a contiguous tensor of the rows' shape, type and device");
+}
+
+void check_status_tensor(const at::Tensor& status, const at::Tensor& x) {
+    TORCH_CHECK(status.is_cuda() && status.device() == x.device() && status.scalar_type() == at::kInt && status.is_contiguous() && status.numel() >= 2,
+                "status must be an int32 tensor on the operands' device");
+}
+
+bool on16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+bool on16(const OptTensor& t) { return !t.has_value() || on16(t->data_ptr()); }
+const void* pointer(const OptTensor& t) { return t.has_value() ? t->data_ptr() : nullptr; }
+int64_t blocks_of(int64_t columns) { return (columns + 127) / 128; }
+int sm_count() { return at::cuda::getCurrentDeviceProperties()->multiProcessorCount; }
+
+void launched(cudaError_t e, const char* what) {
+    TORCH_CHECK(e == cudaSuccess, what, " launch failed: ", cudaGetErrorString(e));
+    PeerWindow::launches += 1;
+}
+
+void check_weight(const at::Tensor& weight, const at::Tensor& x) {
+    TORCH_CHECK(weight.is_cuda() && weight.device() == x.device() && weight.dim() == 1 && weight.is_contiguous() && weight.size(0) == x.size(1),
+                "weight must be a contiguous tensor of hidden entries on the rows' device");
+    TORCH_CHECK(weight.scalar_type() == x.scalar_type() || weight.scalar_type() == at::kFloat, "weight must have the rows' type or be float32");
+}
+
+void check_hidden(const at::Tensor& x) {
+    TORCH_CHECK(x.size(1) >= 1 && x.size(1) <= (int64_t(1) << 28), "rows must have 1 to 2^28 columns");
+    TORCH_CHECK(x.size(0) < (int64_t(1) << 31), "at most 2^31 - 1 rows");
+}
+
+// (y, q, scales, stream, rstd), undefined where not asked for
+std::vector<OptTensor> rms_norm(const at::Tensor& x, const at::Tensor& weight, const OptTensor& residual, double eps, bool quantize, bool keep, bool save) {
+    check_rows(x, "x");
+    check_hidden(x);
+    const int type = row_type(x, "x");
+    check_weight(weight, x);
+    check_like(residual, x, "residual");
+    TORCH_CHECK(eps >= 0, "eps must not be negative");
+    TORCH_CHECK(quantize || keep, "neither the rows nor their 8-bit form is asked for");
+    c10::cuda::CUDAGuard guard(x.device());
+    OptTensor y, q, scales, stream, rstd;
+    if (keep) y = at::empty_like(x);
+    if (quantize) {
+        q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
+        scales = at::empty({x.size(0), blocks_of(x.size(1))}, x.options().dtype(at::kFloat));
+    }
+    if (residual.has_value()) stream = at::empty_like(x);
+    if (save) rstd = at::empty({x.size(0)}, x.options().dtype(at::kFloat));
+    if (x.size(0) > 0) {
+        norm::NormArgs a{};
+        a.x = x.data_ptr();
+        a.residual = pointer(residual);
+        a.weight = weight.data_ptr();
+        a.stream_out = stream.has_value() ? stream->data_ptr() : nullptr;
+        a.y = y.has_value() ? y->data_ptr() : nullptr;
+        a.q = q.has_value() ? static_cast<uint8_t*>(q->data_ptr()) : nullptr;
+        a.scales = scales.has_value() ? scales->data_ptr<float>() : nullptr;
+        a.rstd = rstd.has_value() ? rstd->data_ptr<float>() : nullptr;
+        a.tokens = x.size(0);
+        a.hidden = int(x.size(1));
+        a.eps = float(eps);
+        a.weight_f32 = weight.scalar_type() == at::kFloat;
+        a.aligned = a.hidden % 8 == 0 && on16(a.x) && on16(a.weight) && on16(residual);
+        launched(norm::launch_norm(a, norm::Type(type), sm_count(), c10::cuda::getCurrentCUDAStream()), "rms_norm");
+    }
+    return {y, q, scales, stream, rstd};
+}
+
+std::pair<at::Tensor, at::Tensor> rms_norm_grad(const at::Tensor& grad_y, const at::Tensor& h, const at::Tensor& weight, const at::Tensor& rstd,
+                                                const OptTensor& grad_stream) {
+    check_rows(h, "h");
+    check_hidden(h);
+    const int type = row_type(h, "h");
+    check_weight(weight, h);
+    check_like(grad_y, h, "grad_y");
+    check_like(grad_stream, h, "grad_residual");
+    TORCH_CHECK(rstd.is_cuda() && rstd.device() == h.device() && rstd.scalar_type() == at::kFloat && rstd.is_contiguous() && rstd.dim() == 1 && rstd.size(0) == h.size(0),
+                "rstd must be float32 [tokens] on the rows' device");
+    c10::cuda::CUDAGuard guard(h.device());
+    at::Tensor grad_x = at::empty_like(h);
+    if (h.size(0) == 0) return {grad_x, at::zeros_like(weight)};
+    at::Tensor grad_weight = at::empty_like(weight);
+    const int sms = sm_count();
+    at::Tensor partial = at::empty({norm::grad_blocks(h.size(0), sms), h.size(1)}, h.options().dtype(at::kFloat));
+    norm::NormGradArgs a{};
+    a.grad_y = grad_y.data_ptr();
+    a.h = h.data_ptr();
+    a.weight = weight.data_ptr();
+    a.rstd = rstd.data_ptr<float>();
+    a.grad_stream = pointer(grad_stream);
+    a.grad_x = grad_x.data_ptr();
+    a.partial = partial.data_ptr<float>();
+    a.grad_weight = grad_weight.data_ptr();
+    a.tokens = h.size(0);
+    a.hidden = int(h.size(1));
+    a.weight_f32 = weight.scalar_type() == at::kFloat;
+    a.aligned = a.hidden % 8 == 0 && on16(a.grad_y) && on16(a.h) && on16(a.weight) && on16(grad_stream);
+    launched(norm::launch_norm_grad(a, norm::Type(type), sms, c10::cuda::getCurrentCUDAStream()), "rms_norm_grad");
+    return {grad_x, grad_weight};
+}
+
+std::pair<at::Tensor, at::Tensor> quantize_rows(const at::Tensor& x) {
+    check_rows(x, "x");
+    check_hidden(x);
+    const int type = row_type(x, "x");
+    c10::cuda::CUDAGuard guard(x.device());
+    at::Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
+    at::Tensor scales = at::empty({x.size(0), blocks_of(x.size(1))}, x.options().dtype(at::kFloat));
+    if (x.size(0) > 0) {
+        norm::QuantizeArgs a{};
+        a.x = x.data_ptr();
+        a.q = static_cast<uint8_t*>(q.data_ptr());
+        a.scales = scales.data_ptr<float>();
+        a.rows = x.size(0);
+        a.columns = int(x.size(1));
+        a.aligned = a.columns % 8 == 0 && on16(a.x);
+        launched(norm::launch_quantize(a, norm::Type(type), c10::cuda::getCurrentCUDAStream()), "quantize_rows");
+    }
+    return {q, scales};
+}
+
+// ------------------------------------------------------------------------------------------------ token order
+
+// (slots, slot_map, expert_counts, expert_offsets)
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> plan_tokens(const at::Tensor& topk_idx, int64_t experts, int64_t alignment, const at::Tensor& status) {
+    TORCH_CHECK(topk_idx.is_cuda() && topk_idx.scalar_type() == at::kLong && topk_idx.dim() == 2 && topk_idx.is_contiguous(),
+                "topk_idx must be a contiguous int64 CUDA tensor [tokens, topk]");
+    TORCH_CHECK(topk_idx.size(1) >= 1 && topk_idx.size(1) <= order::kMaxTopk, "topk must be 1 to 32");
+    TORCH_CHECK(experts >= 1 && experts <= order::kMaxExperts, "num_experts must be 1 to 1024");
+    TORCH_CHECK(alignment >= 1 && alignment <= 4096, "alignment must be 1 to 4096");
+    check_status_tensor(status, topk_idx);
+    const int64_t choices = topk_idx.numel();
+    TORCH_CHECK(choices < (int64_t(1) << 30), "at most 2^30 choices");
+    // every choice has a row whatever the routing: no more than min(experts, choices) ranges are rounded up
+    const int64_t capacity = (choices + std::min(experts, choices) * (alignment - 1)) / alignment * alignment;
+    c10::cuda::CUDAGuard guard(topk_idx.device());
+    const at::TensorOptions i32 = topk_idx.options().dtype(at::kInt);
+    at::Tensor slots = at::empty(topk_idx.sizes(), i32), slot_map = at::empty({capacity}, i32);
+    at::Tensor counts = at::empty({experts}, topk_idx.options()), offsets = at::empty({experts + 1}, topk_idx.options());
+    order::PlanArgs a{};
+    a.topk_idx = topk_idx.data_ptr<int64_t>();
+    a.slots = slots.data_ptr<int>();
+    a.slot_map = slot_map.data_ptr<int>();
+    a.expert_counts = counts.data_ptr<int64_t>();
+    a.expert_offsets = offsets.data_ptr<int64_t>();
+    a.choices = choices;
+    a.capacity = capacity;
+    a.experts = int(experts);
+    a.alignment = alignment;
+    a.status = reinterpret_cast<uint32_t*>(status.data_ptr<int>());
+    launched(order::launch_plan(a, c10::cuda::getCurrentCUDAStream()), "plan_tokens");
+    return {slots, slot_map, counts, offsets};
+}
+
+void check_order(const at::Tensor& slots, const at::Tensor& slot_map, const at::Tensor& x) {
+    TORCH_CHECK(slots.is_cuda() && slots.device() == x.device() && slots.scalar_type() == at::kInt && slots.dim() == 2 && slots.is_contiguous() &&
+                    slots.size(1) >= 1 && slots.size(1) <= order::kMaxTopk,
+                "the order's slots must be contiguous int32 [tokens, topk] on the rows' device");
+    TORCH_CHECK(slot_map.is_cuda() && slot_map.device() == x.device() && slot_map.scalar_type() == at::kInt && slot_map.dim() == 1 &&
+                    slot_map.is_contiguous() && slot_map.size(0) < (int64_t(1) << 31),
+                "the order's slot_map must be contiguous int32 [capacity] on the rows' device");
+}
+
+std::pair<at::Tensor, OptTensor> sort_tokens(const at::Tensor& x, const at::Tensor& slots, const at::Tensor& slot_map, const OptTensor& scales, bool zero_padding) {
+    check_rows(x, "x");
+    check_hidden(x);
+    check_order(slots, slot_map, x);
+    TORCH_CHECK(slots.size(0) == x.size(0), "x and the order must have the same tokens");
+    const auto s = x.scalar_type();
+    TORCH_CHECK(s == at::kBFloat16 || s == at::kHalf || s == at::kFloat || s == at::kFloat8_e4m3fn, "x must be bfloat16, float16, float32 or float8_e4m3fn");
+    if (scales.has_value())
+        TORCH_CHECK(scales->is_cuda() && scales->device() == x.device() && scales->scalar_type() == at::kFloat && scales->dim() == 2 && scales->is_contiguous() &&
+                        scales->size(0) == x.size(0) && scales->size(1) >= 1,
+                    "scales must be contiguous float32 [tokens, blocks] on the rows' device");
+    c10::cuda::CUDAGuard guard(x.device());
+    const int64_t capacity = slot_map.size(0);
+    at::Tensor rows = at::empty({capacity, x.size(1)}, x.options());
+    OptTensor row_scales;
+    if (scales.has_value()) row_scales = at::empty({capacity, scales->size(1)}, scales->options());
+    order::SortArgs a{};
+    a.x = x.data_ptr();
+    a.rows = rows.data_ptr();
+    if (scales.has_value()) {
+        a.extra = scales->data_ptr();
+        a.extra_rows = row_scales->data_ptr();
+        a.extra_bytes = scales->size(1) * 4;
+    }
+    a.slots = slots.data_ptr<int>();
+    a.slot_map = slot_map.data_ptr<int>();
+    a.tokens = x.size(0);
+    a.capacity = capacity;
+    a.topk = int(slots.size(1));
+    a.row_bytes = x.size(1) * x.element_size();
+    a.zero_padding = zero_padding;
+    if (capacity > 0) launched(order::launch_sort(a, c10::cuda::getCurrentCUDAStream()), "sort_tokens");
+    return {rows, row_scales};
+}
+
+void check_gate(const OptTensor& weights, const at::Tensor& slots) {
+    if (weights.has_value())
+        TORCH_CHECK(weights->is_cuda() && weights->device() == slots.device() && weights->scalar_type() == at::kFloat && weights->sizes() == slots.sizes() &&
+                        weights->is_contiguous(),
+                    "weights must be contiguous float32 [tokens, topk] on the rows' device");
+}
+
+at::Tensor unsort_tokens(const at::Tensor& y, const at::Tensor& slots, const at::Tensor& slot_map, const OptTensor& weights, const OptTensor& bias) {
+    check_rows(y, "y");
+    check_hidden(y);
+    const int type = row_type(y, "y");
+    check_order(slots, slot_map, y);
+    TORCH_CHECK(y.size(0) == slot_map.size(0), "y must have a row for every slot of the order");
+    check_gate(weights, slots);
+    if (bias.has_value())
+        TORCH_CHECK(bias->is_cuda() && bias->device() == y.device() && bias->scalar_type() == y.scalar_type() && bias->dim() == 2 && bias->is_contiguous() &&
+                        bias->size(0) == slots.size(0) && bias->size(1) == y.size(1),
+                    "bias must be a contiguous [tokens, hidden] tensor of y's type and device");
+    c10::cuda::CUDAGuard guard(y.device());
+    at::Tensor out = at::empty({slots.size(0), y.size(1)}, y.options());
+    if (slots.size(0) == 0) return out;
+    order::UnsortArgs a{};
+    a.y = y.data_ptr();
+    a.slots = slots.data_ptr<int>();
+    a.weights = static_cast<const float*>(pointer(weights));
+    a.bias = pointer(bias);
+    a.out = out.data_ptr();
+    a.tokens = slots.size(0);
+    a.capacity = y.size(0);
+    a.topk = int(slots.size(1));
+    a.hidden = int(y.size(1));
+    a.aligned = a.hidden % 8 == 0 && on16(a.y) && on16(bias);
+    launched(order::launch_unsort(a, order::Type(type), c10::cuda::getCurrentCUDAStream()), "unsort_tokens");
+    return out;
+}
+
+std::pair<at::Tensor, OptTensor> unsort_tokens_grad(const at::Tensor& grad_out, const at::Tensor& y, const at::Tensor& slots, const at::Tensor& slot_map,
+                                                    const OptTensor& weights) {
+    check_rows(y, "y");
+    check_rows(grad_out, "grad_out");
+    check_hidden(y);
+    const int type = row_type(y, "y");
+    check_order(slots, slot_map, y);
+    check_gate(weights, slots);
+    TORCH_CHECK(y.size(0) == slot_map.size(0), "y must have a row for every slot of the order");
+    TORCH_CHECK(grad_out.device() == y.device() && grad_out.scalar_type() == y.scalar_type() && grad_out.size(0) == slots.size(0) && grad_out.size(1) == y.size(1),
+                "grad_out must be a contiguous [tokens, hidden] tensor of y's type and device");
+    c10::cuda::CUDAGuard guard(y.device());
+    at::Tensor grad_y = at::empty_like(y);
+    OptTensor grad_weights;
+    if (weights.has_value()) grad_weights = at::empty_like(*weights);
+    order::UnsortGradArgs a{};
+    a.grad_out = grad_out.data_ptr();
+    a.y = y.data_ptr();
+    a.slots = slots.data_ptr<int>();
+    a.slot_map = slot_map.data_ptr<int>();
+    a.weights = static_cast<const float*>(pointer(weights));
+    a.grad_y = grad_y.data_ptr();
+    a.grad_weights = grad_weights.has_value() ? grad_weights->data_ptr<float>() : nullptr;
+    a.tokens = slots.size(0);
+    a.capacity = y.size(0);
+    a.topk = int(slots.size(1));
+    a.hidden = int(y.size(1));
+    a.aligned = a.hidden % 8 == 0 && on16(a.grad_out) && on16(a.y);
+    if (a.tokens + a.capacity > 0) launched(order::launch_unsort_grad(a, order::Type(type), c10::cuda::getCurrentCUDAStream()), "unsort_tokens_grad");
+    return {grad_y, grad_weights};
+}
+
+// ------------------------------------------------------------------------------------------------ product
+
+void check_e4m3(const at::Tensor& t, int dims, const char* name) {
+    TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kFloat8_e4m3fn && t.is_contiguous() && t.dim() == dims, name,
+                " must be a contiguous CUDA float8_e4m3fn tensor of the expected rank");
+}
+
+void check_i64(const OptTensor& t, const at::Tensor& a, int64_t entries, const char* name) {
+    if (t.has_value())
+        TORCH_CHECK(t->is_cuda() && t->device() == a.device() && t->scalar_type() == at::kLong && t->is_contiguous() && t->dim() == 1 && t->size(0) == entries, name,
+                    " must be a contiguous int64 tensor of ", std::to_string(entries), " entries on the rows' device");
+}
+
+// (out) or (q, scales)
+std::vector<at::Tensor> grouped_gemm_fp8(const at::Tensor& a, const at::Tensor& a_scales, const at::Tensor& w, const at::Tensor& w_scales,
+                                         const OptTensor& expert_offsets, const OptTensor& expert_counts, const OptTensor& row_scale, bool swiglu, bool quantize,
+                                         int64_t max_expert_rows, const at::Tensor& status) {
+    check_e4m3(a, 2, "a");
+    check_e4m3(w, 3, "w");
+    const int64_t rows = a.size(0), K = a.size(1), E = w.size(0), halves = swiglu ? 2 : 1;
+    TORCH_CHECK(w.device() == a.device() && w.size(2) == K, "w must be [experts, N, K] with the rows' K on the rows' device");
+    TORCH_CHECK(E >= 1 && E <= fp8::kMaxExperts, "w must hold 1 to 1024 experts");
+    TORCH_CHECK(w.size(1) % halves == 0, "w must be [experts, 2 * I, K] with swiglu");
+    const int64_t n = w.size(1) / halves;
+    TORCH_CHECK(K >= 16 && K % 16 == 0 && K < (int64_t(1) << 24), "K must be a multiple of 16 below 2^24");
+    TORCH_CHECK(n >= 16 && n % 16 == 0 && n < (int64_t(1) << 24), "the output's columns must be a multiple of 16 below 2^24");
+    TORCH_CHECK(rows < (int64_t(1) << 31) - 256 && E * w.size(1) < (int64_t(1) << 31), "at most 2^31 - 257 rows and 2^31 - 1 weight rows");
+    const int64_t kb = blocks_of(K), nb = blocks_of(n);
+    TORCH_CHECK(a_scales.is_cuda() && a_scales.device() == a.device() && a_scales.scalar_type() == at::kFloat && a_scales.is_contiguous() && a_scales.dim() == 2 &&
+                    a_scales.size(0) == rows && a_scales.size(1) == kb,
+                "a_scales must be contiguous float32 [rows, ceil(K / 128)] on the rows' device");
+    TORCH_CHECK(w_scales.is_cuda() && w_scales.device() == a.device() && w_scales.scalar_type() == at::kFloat && w_scales.is_contiguous() && w_scales.dim() == 3 &&
+                    w_scales.size(0) == E && w_scales.size(1) == halves * nb && w_scales.size(2) == kb,
+                "w_scales must be contiguous float32 [experts, ceil(N / 128) (of each half with swiglu), ceil(K / 128)] on the rows' device");
+    TORCH_CHECK(on16(a.data_ptr()) && on16(w.data_ptr()), "a and w must lie on 16-byte boundaries");
+    TORCH_CHECK(expert_offsets.has_value() || E == 1, "expert_offsets is needed for more than one expert");
+    check_i64(expert_offsets, a, E + 1, "expert_offsets");
+    check_i64(expert_counts, a, E, "expert_counts");
+    if (row_scale.has_value())
+        TORCH_CHECK(!swiglu && row_scale->is_cuda() && row_scale->device() == a.device() && row_scale->scalar_type() == at::kFloat && row_scale->is_contiguous() &&
+                        row_scale->dim() == 1 && row_scale->size(0) == rows,
+                    "row_scale must be contiguous float32 [rows] on the rows' device (without swiglu)");
+    TORCH_CHECK(max_expert_rows >= 0, "max_expert_rows must not be negative");
+    check_status_tensor(status, a);
+    c10::cuda::CUDAGuard guard(a.device());
+    std::vector<at::Tensor> out;
+    if (quantize) {
+        out.push_back(at::empty({rows, n}, a.options()));
+        out.push_back(at::empty({rows, nb}, a_scales.options()));
+    } else {
+        out.push_back(at::empty({rows, n}, a.options().dtype(at::kBFloat16)));
+    }
+    if (rows == 0) return out;
+    fp8::Args g{};
+    g.a = static_cast<const uint8_t*>(a.data_ptr());
+    g.w = static_cast<const uint8_t*>(w.data_ptr());
+    g.a_scales = a_scales.data_ptr<float>();
+    g.w_scales = w_scales.data_ptr<float>();
+    g.expert_offsets = static_cast<const int64_t*>(pointer(expert_offsets));
+    g.expert_counts = static_cast<const int64_t*>(pointer(expert_counts));
+    g.row_scale = static_cast<const float*>(pointer(row_scale));
+    if (quantize) {
+        g.q = static_cast<uint8_t*>(out[0].data_ptr());
+        g.scales = out[1].data_ptr<float>();
+    } else {
+        g.out = reinterpret_cast<__nv_bfloat16*>(out[0].data_ptr());
+    }
+    g.rows = rows;
+    g.experts = int(E);
+    g.k = int(K);
+    g.n = int(n);
+    g.k_blocks = int(kb);
+    g.n_blocks = int(nb);
+    g.swiglu = swiglu;
+    g.status = reinterpret_cast<uint32_t*>(status.data_ptr<int>());
+    launched(fp8::launch(g, sm_count(), c10::cuda::getCurrentCUDAStream()), "grouped_gemm_fp8");
+    return out;
+}
+
+}  // namespace
+
+void bind_ops(pybind11::module_& m) {
+    namespace py = pybind11;
+    m.def("rms_norm", &rms_norm, py::arg("x"), py::arg("weight"), py::arg("residual"), py::arg("eps"), py::arg("quantize"), py::arg("keep"), py::arg("save"));
+    m.def("rms_norm_grad", &rms_norm_grad, py::arg("grad_y"), py::arg("h"), py::arg("weight"), py::arg("rstd"), py::arg("grad_stream"));
+    m.def("quantize_rows", &quantize_rows, py::arg("x"));
+    m.def("plan_tokens", &plan_tokens, py::arg("topk_idx"), py::arg("num_experts"), py::arg("alignment"), py::arg("status"));
+    m.def("sort_tokens", &sort_tokens, py::arg("x"), py::arg("slots"), py::arg("slot_map"), py::arg("scales"), py::arg("zero_padding"));
+    m.def("unsort_tokens", &unsort_tokens, py::arg("y"), py::arg("slots"), py::arg("slot_map"), py::arg("weights"), py::arg("bias"));
+    m.def("unsort_tokens_grad", &unsort_tokens_grad, py::arg("grad_out"), py::arg("y"), py::arg("slots"), py::arg("slot_map"), py::arg("weights"));
+    m.def("grouped_gemm_fp8", &grouped_gemm_fp8, py::arg("a"), py::arg("a_scales"), py::arg("w"), py::arg("w_scales"), py::arg("expert_offsets"),
+          py::arg("expert_counts"), py::arg("row_scale"), py::arg("swiglu"), py::arg("quantize"), py::arg("max_expert_rows"), py::arg("status"));
+}
+
+}  // namespace nep

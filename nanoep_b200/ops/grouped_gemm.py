@@ -30,14 +30,34 @@ def status_tensor(device) -> torch.Tensor:
     return _status[index]
 
 
+def operator_status(x: torch.Tensor) -> torch.Tensor:
+    """``status_tensor`` of a tensor's device for operators that can be captured: it must exist before a capture starts."""
+    found = _status.get(x.device.index) if x.is_cuda else None
+    if found is not None:
+        return found
+    if not x.is_cuda:
+        raise ValueError("operands must be CUDA tensors")
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("the first call on a device cannot be captured: call once before the capture, as for any warm-up")
+    return status_tensor(x.device)
+
+
+def refuse_captured_gradients(name: str, explicit: str):
+    """Autograd's accumulation nodes remember the stream of the graph that made them; one that outlives into a capture ends the process.
+    The explicit gradient functions have no such nodes."""
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{name} is not differentiated inside a CUDA graph capture: call {explicit} there")
+
+
 def check_status(device=None):
-    """Raise if a GEMM kernel on ``device`` gave up on a bounded wait (synchronises)."""
+    """Raise if a kernel of these operators on ``device`` gave up on a bounded wait or met invalid indices (synchronises)."""
     st = status_tensor(device if device is not None else torch.cuda.current_device())
     code, cta = (int(v) for v in st[:2].tolist())
     if code != 0:
         st.zero_()
         reasons = {101: "an operand pipeline wait timed out", 102: "the wait for a row block's ready counter timed out",
-                   103: "expert_offsets are not multiples of 128 from 0 to the row count", 104: "handle metadata names an impossible rank, token or row"}
+                   103: "expert_offsets are not multiples of 128 from 0 to the row count", 104: "handle metadata names an impossible rank, token or row",
+                   105: "an expert id lies outside [-1, num_experts)", 106: "expert_offsets fall, do not start at 0 or end behind the rows"}
         raise RuntimeError(f"nanoep_b200 grouped GEMM status {code} ({reasons.get(code, 'unknown')}), detail {cta}")
 
 

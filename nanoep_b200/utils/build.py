@@ -33,6 +33,10 @@ SOURCES = (
     "grouped_gemm_sm100.cu",
     "grouped_gemm_sm100_2cta.cu",
     "expert_gemm_sm100.cu",
+    "op_bindings.cpp",
+    "rms_norm.cu",
+    "token_order.cu",
+    "fp8_gemm_sm100.cu",
 )
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -1,0 +1,131 @@
+"""The layer with experts in 8 bits: norm, order, products and back as they are used together.
+
+Tolerance: held in 8 bits between its steps, a value is off by 2^-4 at most, the root of the mean square of a rounding within its step by
+about 2^-4 / sqrt(3) = 0.036 at the coarse end of a binade.  The reference makes the same roundings from 64-bit sums; where a value lies next to a border
+the layer's 32-bit sum may fall on the other side, an error of one step of one value in thousands.  2-norm of the difference below 0.02 of
+the result leaves room for the bf16 roundings (2^-8 each) and for those; a missing or doubled row shows as a multiple of it."""
+
+import pytest
+import torch
+
+from nanoep_b200.models.quantized_moe import QuantizedMoE
+from nanoep_b200.ops import grouped_gemm as gg
+from nanoep_b200.ops.rms_norm import rms_norm
+
+pytestmark = pytest.mark.gpu
+
+
+def _blockwise(v):
+    """64-bit values held in e4m3 with a scale for each 128 columns."""
+    n = v.shape[1]
+    blocks = torch.nn.functional.pad(v, (0, -n % 128)).view(len(v), -1, 128)
+    most = blocks.abs().amax(-1, keepdim=True).clamp_min(1e-30)
+    return ((blocks * 448 / most).to(torch.float8_e4m3fn).double() * (most / 448)).view(len(v), -1)[:, :n]
+
+
+def _full(w, scales, halves):
+    E, n, k = w.shape
+    s = scales.double().view(E, halves, -1, scales.shape[-1]).repeat_interleave(128, 2)[:, :, : n // halves].repeat_interleave(128, 3)[..., :k]
+    return w.double() * s.reshape(E, n, k)
+
+
+def _reference(layer, x, idx, gate, residual):
+    h = x if residual is None else (x.float() + residual.float()).to(x.dtype)
+    v = h.double() * layer.norm_weight.double() if layer.norm_weight is not None else h.double()
+    n = _blockwise(v)
+    if layer.norm_weight is not None:
+        n = n * (h.double().square().mean(-1, keepdim=True) + layer.eps).rsqrt()
+    w13, w2 = _full(layer.w13, layer.w13_scales, 2), _full(layer.w2, layer.w2_scales, 1)
+    out = torch.zeros(x.shape, dtype=torch.float64, device="cuda")
+    for e in range(layer.num_experts):
+        t, k = (idx == e).nonzero(as_tuple=True)
+        if len(t):
+            g, u = (n[t] @ w13[e].T).chunk(2, 1)
+            y = (_blockwise(g * torch.sigmoid(g) * u) @ w2[e].T).to(torch.bfloat16).double()
+            out.index_add_(0, t, y * gate[t, k].double()[:, None])
+    return out, h
+
+
+def _layer(experts, hidden, inner, norm=True):
+    gen = torch.Generator(device="cuda").manual_seed(hidden)
+    w13 = torch.randn(experts, 2 * inner, hidden, generator=gen, device="cuda") * hidden**-0.5
+    w2 = torch.randn(experts, hidden, inner, generator=gen, device="cuda") * inner**-0.5
+    weight = (torch.rand(hidden, generator=gen, device="cuda") + 0.5).to(torch.bfloat16) if norm else None
+    return QuantizedMoE.quantize(w13.to(torch.bfloat16), w2.to(torch.bfloat16), norm_weight=weight)
+
+
+def _batch(tokens, hidden, experts, topk, seed=0, masked=True):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(tokens, hidden, generator=gen, device="cuda").to(torch.bfloat16)
+    gate, idx = torch.rand(tokens, experts, generator=gen, device="cuda").topk(topk, dim=-1)
+    if masked:
+        idx = idx.masked_fill(torch.rand(tokens, topk, generator=gen, device="cuda") < 0.2, -1)
+    return x, idx, gate / gate.sum(-1, keepdim=True)
+
+
+def _near(got, want):
+    assert bool(got.isfinite().all())
+    assert float((got.double() - want).norm()) <= 0.02 * float(want.norm())
+
+
+@pytest.mark.parametrize("tokens,hidden,inner,experts,topk", [(1, 256, 128, 4, 2), (33, 512, 256, 8, 4), (200, 1040, 400, 3, 2), (7, 2048, 512, 64, 6), (600, 768, 384, 2, 2)])
+@pytest.mark.parametrize("norm", [True, False])
+def test_layer(tokens, hidden, inner, experts, topk, norm):
+    layer = _layer(experts, hidden, inner, norm)
+    x, idx, gate = _batch(tokens, hidden, experts, topk)
+    out = layer(x, idx, gate)
+    want, _ = _reference(layer, x, idx, gate, None)
+    _near(out, want)
+    bias = torch.randn(tokens, hidden, device="cuda").to(torch.bfloat16)
+    _near(layer(x, idx, gate, bias=bias), want + bias.double())
+    if norm:
+        residual = torch.randn(tokens, hidden, device="cuda").to(torch.bfloat16)
+        out, stream = layer(x, idx, gate, residual=residual)
+        want, h = _reference(layer, x, idx, gate, residual)
+        _near(out, want)
+        assert torch.equal(stream, h)
+    gg.check_status()
+
+
+def test_router_sees_the_normed_rows():
+    layer = _layer(8, 512, 256)
+    x, idx, gate = _batch(40, 512, 8, 2, masked=False)
+    seen = []
+    out = layer(x, router=lambda rows: (seen.append(rows), (idx, gate))[1])
+    assert torch.equal(seen[0], rms_norm(x, layer.norm_weight, eps=layer.eps).y)
+    assert torch.equal(out, layer(x, idx, gate))
+
+
+def test_every_choice_masked():
+    layer = _layer(4, 256, 128)
+    x = torch.randn(5, 256, device="cuda").to(torch.bfloat16)
+    out = layer(x, torch.full((5, 2), -1, device="cuda"), torch.full((5, 2), float("nan"), device="cuda"))
+    assert not out.any()
+
+
+def test_captured_step():
+    layer = _layer(8, 512, 256)
+    x, idx, gate = _batch(64, 512, 8, 4)
+    residual = torch.randn_like(x)
+    layer(x, idx, gate, residual=residual)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = layer(x, idx, gate, residual=residual)
+    for seed in (1, 2):
+        for mine, new in zip((x, idx, gate), _batch(64, 512, 8, 4, seed)):
+            mine.copy_(new)
+        graph.replay()
+        again = layer(x, idx, gate, residual=residual)
+        assert torch.equal(held[0], again[0]) and torch.equal(held[1], again[1])
+
+
+def test_refusals():
+    layer = _layer(4, 256, 128)
+    with pytest.raises(ValueError):
+        QuantizedMoE(layer.w13, layer.w13_scales, layer.w2[:, :128], layer.w2_scales)
+    with pytest.raises(ValueError):
+        QuantizedMoE(layer.w13.float(), layer.w13_scales, layer.w2, layer.w2_scales)
+    with pytest.raises(ValueError):
+        bare = QuantizedMoE(layer.w13, layer.w13_scales, layer.w2, layer.w2_scales)
+        x, idx, gate = _batch(4, 256, 4, 2)
+        bare(x, idx, gate, residual=x)

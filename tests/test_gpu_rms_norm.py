@@ -1,0 +1,205 @@
+"""Norm with the residual's addition and the 8-bit output, against the formula in 64 bits.
+
+Tolerances.  A rounding to type t is off by at most eps(t) / 2 relative.  In 32 bits: the sum of squares of H <= 40000 values is added in
+chains of at most H / 512 + 21 (a thread's columns, the warp, the warps), under 2^-24 each, halved by the root; rsqrtf and the two
+products add under 2^-21: together below 2^-17 for every H here.
+"""
+
+import pytest
+import torch
+
+from nanoep_b200.ops.fp8_gemm import quantize_rows
+from nanoep_b200.ops.rms_norm import rms_norm, rms_norm_grad
+
+pytestmark = pytest.mark.gpu
+EPS32 = 2.0**-17
+SMALLEST = {torch.bfloat16: 2.0**-126, torch.float16: 2.0**-24, torch.float32: 2.0**-126}
+
+
+def _half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def _reference(x, weight, residual, eps):
+    h = x if residual is None else (x.float() + residual.float()).to(x.dtype)
+    v = h.double() * weight.double()
+    rstd = (h.double().square().mean(-1, keepdim=True) + eps).rsqrt()
+    return h, v, rstd
+
+
+def _blocks(v):
+    pad = -v.shape[1] % 128
+    return torch.nn.functional.pad(v, (0, pad)).view(v.shape[0], -1, 128)
+
+
+def _check_quantized(q, scales, v, rstd, exact):
+    """q against v * 448 / max |v|; bit for bit where v is a product of two 16-bit values: the quotient in 32 bits is a tie only where it is one."""
+    blocks = _blocks(v)
+    most = blocks.abs().amax(-1).clamp_min(1e-30)
+    want = (blocks * 448 / most[..., None]).view(v.shape[0], -1)[:, : v.shape[1]]
+    torch.testing.assert_close(scales.double(), most * rstd / 448, rtol=EPS32, atol=0)
+    if exact:
+        assert torch.equal(q.float(), want.to(torch.float8_e4m3fn).float())
+    else:
+        # half a step of e4m3 (2^-4 relative, 2^-10 among the denormals) around a quotient that is off by 2^-22 at most
+        assert bool(((q.double() - want).abs() <= want.abs() * (2.0**-4 + 2.0**-21) + 2.0**-10).all())
+
+
+@pytest.mark.parametrize("tokens,hidden", [(1, 128), (1, 7168), (3, 8), (5, 1000), (2, 1), (7, 129), (33, 4096), (2, 8200), (2, 16392), (3, 40000), (700, 520)])
+@pytest.mark.parametrize("dtype,wide", [(torch.bfloat16, False), (torch.bfloat16, True), (torch.float16, False), (torch.float16, True), (torch.float32, False)])
+@pytest.mark.parametrize("with_residual", [False, True])
+def test_forward(tokens, hidden, dtype, wide, with_residual):
+    torch.manual_seed(tokens * hidden)
+    x = torch.randn(tokens, hidden, device="cuda").to(dtype)
+    residual = (torch.randn(tokens, hidden, device="cuda") * 3).to(dtype) if with_residual else None
+    weight = (torch.randn(hidden, device="cuda") * 0.3 + 1).to(torch.float32 if wide else dtype)
+    got = rms_norm(x, weight, residual=residual, eps=1e-5, quantize=True, save=True)
+    h, v, rstd = _reference(x, weight, residual, 1e-5)
+    if with_residual:
+        assert torch.equal(got.residual, h)
+    else:
+        assert got.residual is None
+    torch.testing.assert_close(got.rstd.double(), rstd[:, 0], rtol=EPS32, atol=0)
+    torch.testing.assert_close(got.y.double(), v * rstd, rtol=_half_step(dtype) + 2 * EPS32, atol=SMALLEST[dtype])
+    _check_quantized(got.q, got.scales, v, rstd, exact=dtype != torch.float32 and not wide)
+    alone = rms_norm(x, weight, residual=residual, eps=1e-5)
+    only = rms_norm(x, weight, residual=residual, eps=1e-5, quantize=True, keep=False)
+    assert alone.q is None and only.y is None and torch.equal(alone.y, got.y)
+    assert torch.equal(only.q.view(torch.uint8), got.q.view(torch.uint8)) and torch.equal(only.scales, got.scales)
+
+
+def test_rows_that_do_not_start_on_16_bytes():
+    x = torch.randn(4, 256, device="cuda").to(torch.bfloat16)
+    shifted = torch.empty(4 * 256 + 1, device="cuda", dtype=torch.bfloat16)[1:].view(4, 256)
+    shifted.copy_(x)
+    weight = torch.randn(256, device="cuda").to(torch.bfloat16)
+    a, b = (rms_norm(t, weight, quantize=True) for t in (x, shifted))
+    # the two kernels add the squares in another order: y may round the other way, the 8-bit values do not depend on the sum
+    torch.testing.assert_close(a.y.float(), b.y.float(), rtol=2 * _half_step(torch.bfloat16) + 2 * EPS32, atol=0)
+    assert torch.equal(a.q.view(torch.uint8), b.q.view(torch.uint8))
+
+
+def test_zero_rows_infinities_and_nan():
+    x = torch.randn(5, 384, device="cuda").to(torch.bfloat16)
+    x[0] = 0
+    x[1, 7] = float("inf")
+    x[2, 200] = float("nan")
+    x[3, :128] = 0
+    weight = torch.ones(384, device="cuda", dtype=torch.bfloat16)
+    got = rms_norm(x, weight, quantize=True)
+    assert torch.equal(got.y[0], torch.zeros_like(got.y[0])) and not got.q[0].float().any() and bool((got.scales[0] > 0).all())
+    assert bool(got.y[2].isnan().all()) and bool(got.scales[2].isnan().all())
+    assert bool(got.scales[1, 0].isnan()) and bool(got.y[1, 7].isnan()) and not got.y[1, 8:].any()  # rstd is 0
+    assert not got.q[3, :128].float().any() and bool(got.q[3, 128:].float().abs().amax() == 448)
+    assert bool(got.y[4].isfinite().all())
+
+
+@pytest.mark.parametrize("rows,columns", [(1, 128), (1, 16), (3, 129), (5, 8), (257, 4096), (2, 1000), (1, 7)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_quantize_rows(rows, columns, dtype):
+    torch.manual_seed(rows)
+    x = (torch.randn(rows, columns, device="cuda") * torch.logspace(-4, 3, rows, device="cuda")[:, None]).to(dtype)
+    x[0, 0] = 0
+    q, scales = quantize_rows(x)
+    _check_quantized(q, scales, x.double(), torch.ones(rows, 1, device="cuda", dtype=torch.float64), exact=dtype != torch.float32)
+
+
+def _gradients(h, weight, rstd, gy, gh):
+    """The formula's gradients in 64 bits, and the size of what is added up in each."""
+    xhat, gw = h.double() * rstd, gy.double() * weight.double()
+    mean, size = (gw * xhat).mean(-1, keepdim=True), (gw * xhat).abs().mean(-1, keepdim=True)
+    dx = rstd * (gw - xhat * mean)
+    scale = rstd * (gw.abs() + xhat.abs() * size)
+    if gh is not None:
+        dx, scale = dx + gh.double(), scale + gh.double().abs()
+    return dx, scale, (gy.double() * xhat).sum(0), (gy.double() * xhat).abs().sum(0)
+
+
+@pytest.mark.parametrize("tokens,hidden", [(1, 128), (3, 1000), (2, 129), (301, 4096), (900, 512), (5, 16392), (2, 7)])
+@pytest.mark.parametrize("dtype,wide", [(torch.bfloat16, False), (torch.bfloat16, True), (torch.float16, False), (torch.float32, False)])
+@pytest.mark.parametrize("with_residual", [False, True])
+def test_gradients(tokens, hidden, dtype, wide, with_residual):
+    torch.manual_seed(tokens + hidden)
+    x = torch.randn(tokens, hidden, device="cuda").to(dtype).requires_grad_()
+    residual = (torch.randn(tokens, hidden, device="cuda") * 3).to(dtype).requires_grad_() if with_residual else None
+    weight = (torch.randn(hidden, device="cuda") * 0.3 + 1).to(torch.float32 if wide else dtype).requires_grad_()
+    gy = torch.randn(tokens, hidden, device="cuda").to(dtype)
+    gh = torch.randn(tokens, hidden, device="cuda").to(dtype) if with_residual else None
+    got = rms_norm(x, weight, residual=residual, quantize=True)
+    leaves = (x, weight, residual) if with_residual else (x, weight)
+    grads = torch.autograd.grad((got.y, got.residual) if with_residual else got.y, leaves, (gy, gh) if with_residual else gy)
+    with torch.no_grad():
+        h, _, rstd = _reference(x, weight, residual, 1e-6)
+        dx, size, dw, dw_size = _gradients(h, weight, rstd, gy, gh)
+        # dx: 32-bit arithmetic on terms of `size`, one rounding; dw: chains of rows of a block, of blocks and of eight parts
+        assert bool(((grads[0].double() - dx).abs() <= _half_step(dtype) * dx.abs() + 2 * EPS32 * size + SMALLEST[dtype]).all())
+        chain = tokens // 148 + 300 / 8 + 12
+        wt = weight.dtype
+        assert bool(((grads[1].double() - dw).abs() <= _half_step(wt) * dw.abs() + (EPS32 + chain * 2.0**-24) * dw_size + SMALLEST[wt]).all())
+        if with_residual:
+            assert torch.equal(grads[2], grads[0])
+        saved = rms_norm(x, weight, residual=residual, save=True)
+        again = rms_norm_grad(gy, h, weight, saved.rstd, grad_residual=gh)
+        assert torch.equal(again[0], grads[0]) and torch.equal(again[1], grads[1]), "the same sums on every run"
+
+
+def test_gradients_against_differences():
+    """Central differences of the operator itself.  With steps of 2^-6 the third-order term stays below 2^-12 / 6 of the derivative's
+    size times a small factor; the forward's own rounding is 2^-17 of the loss's terms over 2^-5."""
+    torch.manual_seed(1)
+    x, r, w = torch.randn(3, 96, device="cuda"), torch.randn(3, 96, device="cuda"), torch.rand(96, device="cuda") + 0.5
+    gy, gh = torch.randn(3, 96, device="cuda"), torch.randn(3, 96, device="cuda")
+
+    def loss(x, r, w):
+        got = rms_norm(x, w, residual=r)
+        return (got.y.double() * gy).sum() + (got.residual.double() * gh).sum()
+
+    leaves = [t.clone().requires_grad_() for t in (x, r, w)]
+    got = rms_norm(leaves[0], leaves[2], residual=leaves[1])
+    grads = torch.autograd.grad((got.y, got.residual), leaves, (gy, gh))
+    for i, t in enumerate((x, r, w)):
+        d = torch.randn_like(t)
+        d /= d.norm() / 4
+        step = 2.0**-6
+        moved = [[u + s * step * d if j == i else u for j, u in enumerate((x, r, w))] for s in (1, -1)]
+        slope = (loss(*moved[0]) - loss(*moved[1])) / (2 * step)
+        want = (grads[i].double() * d.double()).sum()
+        size = (grads[i].double() * d.double()).abs().sum()
+        noise = 2.0**-17 * (gy.abs().sum() * 3 + gh.abs().sum()) / (2 * step) / 16
+        assert abs(float(slope - want)) <= float(size) * 2.0**-7 + float(noise)
+
+
+def test_gradient_of_the_stream_alone_and_without_rows():
+    x = torch.randn(2, 64, device="cuda", requires_grad=True)
+    r = torch.randn(2, 64, device="cuda")
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    g = torch.randn(2, 64, device="cuda")
+    dx, dw = torch.autograd.grad(rms_norm(x, w, residual=r).residual, (x, w), g, allow_unused=True)
+    assert torch.equal(dx, g) and dw is None
+    empty = torch.empty(0, 64, device="cuda", requires_grad=True)
+    got = rms_norm(empty, w, quantize=True)
+    dx, dw = torch.autograd.grad(got.y, (empty, w), torch.empty(0, 64, device="cuda"))
+    assert got.q.shape == (0, 64) and got.scales.shape == (0, 1) and dx.shape == (0, 64) and not dw.any()
+
+
+def test_refusals():
+    x = torch.randn(2, 64, device="cuda")
+    w = torch.ones(64, device="cuda")
+    for bad in (
+        lambda: rms_norm(x.cpu(), w),
+        lambda: rms_norm(x.t(), w),
+        lambda: rms_norm(x.double(), w),
+        lambda: rms_norm(x, w[:32]),
+        lambda: rms_norm(x, w.to(torch.bfloat16)),
+        lambda: rms_norm(x, w, residual=x.half()),
+        lambda: rms_norm(x, w, residual=x[:1]),
+        lambda: rms_norm(x, w, eps=-1.0),
+        lambda: rms_norm(x, w, keep=False),
+        lambda: rms_norm(x[0], w),
+        lambda: rms_norm_grad(x, x, w, torch.ones(3, device="cuda")),
+        lambda: quantize_rows(x.to(torch.int32)),
+    ):
+        with pytest.raises(RuntimeError):
+            bad()
+    with pytest.raises(ValueError):
+        rms_norm(x.requires_grad_(), w, quantize=True, keep=False)
