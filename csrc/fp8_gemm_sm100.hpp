@@ -11,9 +11,13 @@ namespace fp8 {
 constexpr int kMaxExperts = 1024;
 enum Fp8Status : uint32_t { kPipeTimeout = 101, kBadOffsets = 106 };
 
+// Tensor maps: rows in boxes of 128, 64, 32 and 16 (by 128 columns), weights [experts (* 2)][n][k] in boxes of 128 rows (64 with SwiGLU).
+struct Maps {
+    CUtensorMap weights;
+    CUtensorMap rows[4];
+};
+
 struct Args {
-    const uint8_t* a;               // e4m3 [rows, k]
-    const uint8_t* w;               // e4m3 [experts, (2 *) n, k]
     const float* a_scales;          // [rows, k_blocks]
     const float* w_scales;          // [experts, (2 *) n_blocks, k_blocks]
     const int64_t* expert_offsets;  // [experts + 1], or null: one expert owns all rows
@@ -23,12 +27,14 @@ struct Args {
     uint8_t* q;                     // e4m3 [rows, n] with
     float* scales;                  // [rows, n_blocks]
     int64_t rows;
-    int experts, k, n;              // n: output columns (with SwiGLU half of the weight's rows)
+    int experts, n;                 // n: output columns (with SwiGLU half of the weight's rows)
     int k_blocks, n_blocks;         // of 128
+    int n_tiles;                    // of 256 output columns (128 with SwiGLU)
     int swiglu;
     uint32_t* status;               // 2 words: first error code, detail
+    uint64_t timeout_ns;
 };
-cudaError_t launch(const Args& args, int sms, cudaStream_t stream);
+cudaError_t launch(const Maps& maps, const Args& args, int grid, cudaStream_t stream);
 
 }  // namespace fp8
 }  // namespace nep

@@ -167,7 +167,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> plan_tokens(const at:
     const int64_t choices = topk_idx.numel();
     TORCH_CHECK(choices < (int64_t(1) << 30), "at most 2^30 choices");
     // every choice has a row whatever the routing: no more than min(experts, choices) ranges are rounded up
-    const int64_t capacity = (choices + std::min(experts, choices) * (alignment - 1)) / alignment * alignment;
+    const int64_t capacity = (choices + (std::min(experts, choices) + 1) * (alignment - 1)) / alignment * alignment;
+    TORCH_CHECK(capacity < (int64_t(1) << 31), "at most 2^31 - 1 rows");
     c10::cuda::CUDAGuard guard(topk_idx.device());
     const at::TensorOptions i32 = topk_idx.options().dtype(at::kInt);
     at::Tensor slots = at::empty(topk_idx.sizes(), i32), slot_map = at::empty({capacity}, i32);
@@ -301,6 +302,30 @@ std::pair<at::Tensor, OptTensor> unsort_tokens_grad(const at::Tensor& grad_out, 
 
 // ------------------------------------------------------------------------------------------------ product
 
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// Row-major 8-bit [rows, columns], or [outer, rows, columns]; box = 128 columns (one swizzle row) x box_rows rows.  What a box covers
+// outside of the tensor reads as zero.
+CUtensorMap e4m3_map(const void* base, int64_t columns, int64_t rows, int64_t outer, int box_rows) {
+    static EncodeFn encode = [] {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult result;
+        cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &result);
+        TORCH_CHECK(e == cudaSuccess && result == cudaDriverEntryPointSuccess && ptr != nullptr, "cuTensorMapEncodeTiled is not available");
+        return reinterpret_cast<EncodeFn>(ptr);
+    }();
+    CUtensorMap map;
+    const cuuint64_t dims[3] = {cuuint64_t(columns), cuuint64_t(rows), cuuint64_t(outer)};
+    const cuuint64_t strides[2] = {cuuint64_t(columns), cuuint64_t(rows) * cuuint64_t(columns)};
+    const cuuint32_t box[3] = {128, cuuint32_t(box_rows), 1};
+    const cuuint32_t elem[3] = {1, 1, 1};
+    const CUresult r = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, outer > 0 ? 3 : 2, const_cast<void*>(base), dims, strides, box, elem,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed");
+    return map;
+}
+
 void check_e4m3(const at::Tensor& t, int dims, const char* name) {
     TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kFloat8_e4m3fn && t.is_contiguous() && t.dim() == dims, name,
                 " must be a contiguous CUDA float8_e4m3fn tensor of the expected rank");
@@ -352,9 +377,10 @@ std::vector<at::Tensor> grouped_gemm_fp8(const at::Tensor& a, const at::Tensor& 
         out.push_back(at::empty({rows, n}, a.options().dtype(at::kBFloat16)));
     }
     if (rows == 0) return out;
+    fp8::Maps maps{};
+    maps.weights = e4m3_map(w.data_ptr(), K, n, E * halves, swiglu ? 64 : 128);
+    for (int b = 0; b < 4; ++b) maps.rows[b] = e4m3_map(a.data_ptr(), K, rows, 0, 128 >> b);
     fp8::Args g{};
-    g.a = static_cast<const uint8_t*>(a.data_ptr());
-    g.w = static_cast<const uint8_t*>(w.data_ptr());
     g.a_scales = a_scales.data_ptr<float>();
     g.w_scales = w_scales.data_ptr<float>();
     g.expert_offsets = static_cast<const int64_t*>(pointer(expert_offsets));
@@ -368,13 +394,16 @@ std::vector<at::Tensor> grouped_gemm_fp8(const at::Tensor& a, const at::Tensor& 
     }
     g.rows = rows;
     g.experts = int(E);
-    g.k = int(K);
     g.n = int(n);
     g.k_blocks = int(kb);
     g.n_blocks = int(nb);
+    g.n_tiles = int(swiglu ? nb : (nb + 1) / 2);
     g.swiglu = swiglu;
     g.status = reinterpret_cast<uint32_t*>(status.data_ptr<int>());
-    launched(fp8::launch(g, sm_count(), c10::cuda::getCurrentCUDAStream()), "grouped_gemm_fp8");
+    g.timeout_ns = uint64_t(5e9);
+    // a cluster for every tile that the rows allow, as far as the GPU holds them
+    const int64_t tiles = (rows / 256 + std::min(E, rows)) * g.n_tiles;
+    launched(fp8::launch(maps, g, int(std::min<int64_t>(sm_count(), 2 * tiles)), c10::cuda::getCurrentCUDAStream()), "grouped_gemm_fp8");
     return out;
 }
 

@@ -32,7 +32,7 @@ class TokenOrder(NamedTuple):
 def plan_tokens(topk_idx: torch.Tensor, num_experts: int, *, alignment: int = 1) -> TokenOrder:
     """Order of the choices ``topk_idx`` (int64 ``[T, K]``, expert ids or -1) by expert.
 
-    Capacity is ``T * K + min(E, T * K) * (alignment - 1)``, rounded down to a multiple of ``alignment``.  An id outside ``[-1, E)`` is
+    Capacity is ``T * K + min(E, T * K) * (alignment - 1)``, rounded up to a multiple of ``alignment``.  An id outside ``[-1, E)`` is
     treated as masked and reported by ``grouped_gemm.check_status()``.
     """
     return TokenOrder(*_ext().plan_tokens(topk_idx, int(num_experts), int(alignment), operator_status(topk_idx)))

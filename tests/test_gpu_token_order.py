@@ -24,7 +24,7 @@ def _order(idx, experts, alignment):
     offsets = [0]
     for c in counts:
         offsets.append(offsets[-1] + -(-c // alignment) * alignment)
-    capacity = (len(choice) + min(experts, len(choice)) * (alignment - 1)) // alignment * alignment
+    capacity = -(-(len(choice) + min(experts, len(choice)) * (alignment - 1)) // alignment) * alignment
     assert offsets[-1] <= capacity
     at, slots, slot_map = offsets[:-1].copy(), [], [-1] * capacity
     for i, e in enumerate(choice):
