@@ -35,18 +35,22 @@ constexpr int kStageBytes = 2 * kHalfBytes;
 constexpr int kStages = 6;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 128 + 32 * kEpiWarps;   // a warpgroup that loads and issues, two that add up
-// A launch of 384 threads gives each 168 registers.  The sums need more: 72 + 2 * 216 = 3 * 168, what the block was launched with.
-constexpr int kFewRegisters = 72, kManyRegisters = 216;
+// A launch of 384 threads gives each 168 registers.  The sums need more: 80 + 2 * 208 < 3 * 168, what the block was launched with.
+constexpr int kFewRegisters = 80, kManyRegisters = 208;
 static_assert(128 * kFewRegisters + 32 * kEpiWarps * kManyRegisters <= kThreads * 168, "registers of the launch");
 constexpr int kTmemCols = 512;
+constexpr int kScaleBlocks = 8;                  // blocks whose scales are loaded at a time: 32 bytes of a row
 // M 256, N 256, e4m3 x e4m3 -> fp32, both operands K-major
 constexpr uint32_t kInstrDesc = (1u << 4) | (uint32_t(kTileCols >> 3) << 17) | (uint32_t((2 * kTileRows) >> 4) << 24);
 
 struct Shared {
     uint64_t full[kStages], empty[kStages], tmem_full[2], tmem_empty[2];
+    uint64_t scale_full[2], scale_empty[2];
     uint64_t told[2][4];               // by epilogue group and quarter: its rows' largest values are in `most`
     uint32_t tmem_base;
     int abort;
+    float row_scales[2][kScaleBlocks][kTileRows];  // of the next blocks, by turns
+    float weight_scales[2][kScaleBlocks][2];       // of the pair's two halves (of the gate and up rows)
     float most[2][2][kTileRows];       // largest of each row's 64 columns, by parity of the tile and epilogue group
     int first_row[kMaxExperts];
     int rows[kMaxExperts];
@@ -54,6 +58,27 @@ struct Shared {
 };
 constexpr size_t kSmemBytes = size_t(kStages) * kStageBytes + sizeof(Shared);
 static_assert(kSmemBytes <= 232448, "shared memory of a CTA");
+
+// Bounded wait that reads the timer only once it has polled for a while: a read takes about a microsecond, and the epilogue waits for
+// every block of 128 columns.
+__device__ __forceinline__ bool wait_block(uint64_t* bar, uint32_t parity, uint64_t limit_ns, const volatile int* abort) {
+    uint64_t start = 0;
+    uint32_t spins = 0;
+    while (!mbar_try(bar, parity)) {
+        if ((++spins & 255u) != 0u) continue;
+        if (*abort) return false;
+        const uint64_t now = timer_ns();
+        if (start == 0) start = now;
+        if (now - start > limit_ns) return false;
+    }
+    return true;
+}
+
+// Arrival without a fence: what it stands for, TMEM columns that have been read, is complete when tcgen05.wait::ld returns.  A releasing
+// arrival of cluster scope waits for the thread's loads in flight as well, the scales of the blocks ahead: 1000 cycles a block.
+__device__ __forceinline__ void arrive_read(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
 
 struct Tile {
     int expert, row0, rows, nt;  // rows: of the pair, at most 256
@@ -82,6 +107,22 @@ __device__ __forceinline__ void mma_pair_e4m3(uint32_t d_tmem, uint64_t a_desc, 
                  "l"(a_desc), "l"(b_desc), "r"(kInstrDesc), "r"(accumulate)
                  : "memory");
 }
+// 16 consecutive fp32 columns of this thread's TMEM lane
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr));
+}
+__device__ __forceinline__ uint64_t pair_of(float f) {
+    uint64_t p;
+    asm("mov.b64 %0, {%1, %1};" : "=l"(p) : "r"(__float_as_uint(f)));
+    return p;
+}
+// two columns at a time: sum += {lo, hi} * f
+__device__ __forceinline__ void fma_pair(uint64_t& sum, uint32_t lo, uint32_t hi, uint64_t f) {
+    asm("{\n .reg .b64 v;\n mov.b64 v, {%1, %2};\n fma.rn.f32x2 %0, v, %3, %0;\n}" : "+l"(sum) : "r"(lo), "r"(hi), "l"(f));
+}
 template <int kRegisters>
 __device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegisters)); }
 template <int kRegisters>
@@ -104,6 +145,10 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
         for (int b = 0; b < 2; ++b) {
             mbar_init(&sh.tmem_full[b], 1);
             mbar_init(&sh.tmem_empty[b], 2 * kEpiWarps);  // leader: the epilogue warps of both CTAs
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&sh.scale_full[b], 1);
+            mbar_init(&sh.scale_empty[b], kEpiWarps);
         }
         for (int q = 0; q < 8; ++q) mbar_init(&sh.told[q >> 2][q & 3], 1);
         sh.abort = 0;
@@ -171,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                 const int both = (t.rows + 15) & ~15, mine = max(0, min(kTileRows, both - int(cta) * kTileRows));
                 const uint32_t bytes = uint32_t(2 * kHalfBytes + both * 128);
                 for (int kb = 0; kb < k_blocks; ++kb) {
-                    if (!mbar_wait(&sh.empty[stage], phase ^ 1u, limit_ns)) {
+                    if (!wait_block(&sh.empty[stage], phase ^ 1u, limit_ns, abort_flag)) {
                         fail(kPipeTimeout);
                         break;
                     }
@@ -218,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
             for (int unit = cluster_id; unit < units && !*abort_flag; unit += num_clusters) {
                 for (int kb = 0; kb < k_blocks; ++kb, ++block) {
                     const int buf = block & 1;
-                    if (!mbar_wait(&sh.tmem_empty[buf], (uint32_t(block >> 1) & 1u) ^ 1u, limit_ns) || !mbar_wait(&sh.full[stage], phase, limit_ns)) {
+                    if (!wait_block(&sh.full[stage], phase, limit_ns, abort_flag) || !wait_block(&sh.tmem_empty[buf], (uint32_t(block >> 1) & 1u) ^ 1u, limit_ns, abort_flag)) {
                         fail(kPipeTimeout);
                         break;
                     }
@@ -237,6 +282,47 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                 }
             }
         }
+    } else if (warp == 2) {
+        // ------------------------------------------------------------------ scales (both CTAs)
+        // Eight blocks at a time and up to sixteen ahead: the epilogue warps have no registers left to wait for memory.
+        constexpr int kHalves = kSwiGLU ? 2 : 1;
+        int chunk = 0;
+        bool ok = true;
+        for (int unit = cluster_id; unit < units && ok; unit += num_clusters) {
+            const Tile t = locate(sh, args.experts, args.n_tiles, unit);
+            // 128 weight rows share a scale: the two halves of the tile, or those of its gate and up rows
+            const int half = lane & 1, block = kSwiGLU ? half * args.n_blocks + t.nt : min(2 * t.nt + half, args.n_blocks - 1);
+            const float* sw = args.w_scales + (int64_t(t.expert) * kHalves * args.n_blocks + block) * k_blocks;
+            const float* sa[4];
+            bool real[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = int(cta) * kTileRows + i * 32 + lane;
+                real[i] = r < t.rows;
+                sa[i] = args.a_scales + (int64_t(t.row0) + r) * k_blocks;
+            }
+            for (int kb0 = 0; kb0 < k_blocks; kb0 += kScaleBlocks, ++chunk) {
+                float v[4][kScaleBlocks];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < kScaleBlocks; ++j) v[i][j] = real[i] && kb0 + j < k_blocks ? sa[i][kb0 + j] : 0.f;
+                const float w = kb0 + (lane >> 1) < k_blocks && lane < 2 * kScaleBlocks ? sw[kb0 + (lane >> 1)] : 0.f;
+                const int slot = chunk & 1;
+                ok = __all_sync(0xffffffffu, wait_block(&sh.scale_empty[slot], (uint32_t(chunk >> 1) & 1u) ^ 1u, limit_ns, abort_flag));
+                if (!ok) {
+                    if (lane == 0) fail(kPipeTimeout);
+                    break;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < kScaleBlocks; ++j) sh.row_scales[slot][j][i * 32 + lane] = v[i][j];
+                if (lane < 2 * kScaleBlocks) sh.weight_scales[slot][lane >> 1][half] = w;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.scale_full[slot]);
+            }
+        }
     }
     } else {
         // ------------------------------------------------------------------ epilogue (both CTAs)
@@ -244,8 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
         const int quarter = warp & 3;        // TMEM lanes [32 * quarter, +32) belong to this warp
         const int group = (warp - 4) >> 2;   // its 128 columns
         const int r = quarter * 32 + lane;   // row of this CTA's tile
-        constexpr int kHalves = kSwiGLU ? 2 : 1;
-        int block = 0, exchanges = 0;
+        int block = 0, chunk = 0, exchanges = 0;
         bool ok = true;
         for (int unit = cluster_id; unit < units && ok; unit += num_clusters) {
             const Tile t = locate(sh, args.experts, args.n_tiles, unit);
@@ -253,48 +338,71 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
             const bool real = in_tile < t.rows;
             const bool any = int(cta) * kTileRows + quarter * 32 < t.rows;  // of this warp's rows
             const int64_t row = int64_t(t.row0) + in_tile;
-            const float* sa = args.a_scales + row * k_blocks;
-            // 128 weight rows that share a scale: the group's own, or (SwiGLU) those of the tile's gate and up rows
-            const int wb = kSwiGLU ? t.nt : t.nt * 2 + group;
+            const int wb = kSwiGLU ? t.nt : t.nt * 2 + group;  // output block of this thread
             const bool inside = wb < args.n_blocks;
-            const float* sw = args.w_scales + (int64_t(t.expert) * kHalves * args.n_blocks + (inside ? wb : 0)) * k_blocks;
-            const float* su = sw + int64_t(args.n_blocks) * k_blocks;
-            float acc[128];
+            uint64_t sum[64];  // pairs of neighbouring columns
 #pragma unroll
-            for (int j = 0; j < 128; ++j) acc[j] = 0.f;
+            for (int j = 0; j < 64; ++j) sum[j] = 0;
             for (int kb = 0; kb < k_blocks; ++kb, ++block) {
                 const int buf = block & 1;
-                const float s = real ? sa[kb] : 0.f;
-                const float s0 = s * sw[kb], s1 = kSwiGLU ? s * su[kb] : s0;
-                ok = __all_sync(0xffffffffu, mbar_wait(&sh.tmem_full[buf], uint32_t(block >> 1) & 1u, limit_ns) && !*abort_flag);
+                const int at = kb % kScaleBlocks, slot = chunk & 1;
+                if (at == 0) {
+                    ok = __all_sync(0xffffffffu, wait_block(&sh.scale_full[slot], uint32_t(chunk >> 1) & 1u, limit_ns, abort_flag));
+                    if (!ok) {
+                        if (lane == 0) fail(kPipeTimeout);
+                        break;
+                    }
+                }
+                const float s = sh.row_scales[slot][at][r];
+                const uint64_t f0 = pair_of(s * sh.weight_scales[slot][at][kSwiGLU ? 0 : group]);
+                const uint64_t f1 = kSwiGLU ? pair_of(s * sh.weight_scales[slot][at][1]) : f0;
+                if (at == kScaleBlocks - 1 || kb == k_blocks - 1) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.scale_empty[slot]);
+                    ++chunk;
+                }
+                ok = __all_sync(0xffffffffu, wait_block(&sh.tmem_full[buf], uint32_t(block >> 1) & 1u, limit_ns, abort_flag));
                 if (!ok) {
                     if (lane == 0) fail(kPipeTimeout);
                     break;
                 }
                 tc_fence_after();
+                auto drained = [&]() {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) arrive_read(map_to_cta(smem_u32(&sh.tmem_empty[buf]), 0));
+                };
                 if (any) {
+                    // the next 16 columns are on their way while these are added
                     const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(buf * kTileCols + group * 128);
+                    uint32_t v[2][16];
+                    tmem_ld16(taddr, v[0]);
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t v[32];
-                        tmem_ld32(taddr + c * 32, v);
+                    for (int c = 0; c < 8; ++c) {
                         tmem_ld_wait();
-                        const float f = c < 2 ? s0 : s1;
+                        if (c < 7) tmem_ld16(taddr + (c + 1) * 16, v[(c + 1) & 1]);
+                        else drained();
+                        const uint64_t f = c < 4 ? f0 : f1;
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) acc[c * 32 + j] = fmaf(__uint_as_float(v[j]), f, acc[c * 32 + j]);
+                        for (int j = 0; j < 8; ++j) fma_pair(sum[c * 8 + j], v[c & 1][2 * j], v[c & 1][2 * j + 1], f);
                     }
+                } else {
+                    drained();
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&sh.tmem_empty[buf]), 0));
             }
             if (!ok) break;
             if (!any) continue;
+            float acc[128];
+#pragma unroll
+            for (int j = 0; j < 64; ++j) {
+                acc[2 * j] = __uint_as_float(uint32_t(sum[j]));
+                acc[2 * j + 1] = __uint_as_float(uint32_t(sum[j] >> 32));
+            }
             constexpr int kCols = kSwiGLU ? 64 : 128;  // output columns of this thread
             const int n0 = kSwiGLU ? t.nt * 128 + group * 64 : t.nt * kTileCols + group * 128;
             if (kSwiGLU) {
 #pragma unroll
-                for (int j = 0; j < 64; ++j) acc[j] = silu(acc[j]) * acc[64 + j];
+                for (int j = 0; j < 64; ++j) acc[j] = __fdividef(acc[j], 1.f + __expf(-acc[j])) * acc[64 + j];
             } else if (args.row_scale != nullptr) {
                 const float f = real ? args.row_scale[row] : 0.f;
 #pragma unroll
@@ -311,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                     sh.most[turn][group][r] = m;
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sh.told[group][quarter]);
-                    ok = __all_sync(0xffffffffu, mbar_wait(&sh.told[group ^ 1][quarter], uint32_t(turn), limit_ns));
+                    ok = __all_sync(0xffffffffu, wait_block(&sh.told[group ^ 1][quarter], uint32_t(turn), limit_ns, abort_flag));
                     if (!ok) {
                         if (lane == 0) fail(kPipeTimeout);
                         break;
@@ -320,6 +428,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                     ++exchanges;
                 }
                 m = max_nan(m, kTiny);
+                const float per = __fdiv_rn(kLargest, m);  // sums do not lie on the border of two e4m3 values: a product will do
                 if (real && (kSwiGLU ? group == 0 : inside)) args.scales[row * args.n_blocks + wb] = __fdiv_rn(m, kLargest);
 #pragma unroll
                 for (int j = 0; j < kCols; j += 16) {
@@ -327,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                     uint32_t q[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        q[i] = pack_e4m3(quotient(acc[j + 4 * i], m), quotient(acc[j + 4 * i + 1], m), quotient(acc[j + 4 * i + 2], m), quotient(acc[j + 4 * i + 3], m));
+                        q[i] = pack_e4m3(acc[j + 4 * i] * per, acc[j + 4 * i + 1] * per, acc[j + 4 * i + 2] * per, acc[j + 4 * i + 3] * per);
                     st_v4(args.q + row * args.n + n0 + j, q[0], q[1], q[2], q[3]);
                 }
             } else {
