@@ -18,6 +18,7 @@
 // final cluster barrier and free their TMEM.
 #include "fp8_gemm_sm100.hpp"
 
+#include "fp8_prim.cuh"
 #include "row_prim.cuh"
 #include "tc_prim.cuh"
 
@@ -39,9 +40,7 @@ constexpr int kThreads = 128 + 32 * kEpiWarps;   // a warpgroup that loads and i
 constexpr int kFewRegisters = 80, kManyRegisters = 208;
 static_assert(128 * kFewRegisters + 32 * kEpiWarps * kManyRegisters <= kThreads * 168, "registers of the launch");
 constexpr int kTmemCols = 512;
-constexpr int kScaleBlocks = 8;                  // blocks whose scales are loaded at a time: 32 bytes of a row
-// M 256, N 256, e4m3 x e4m3 -> fp32, both operands K-major
-constexpr uint32_t kInstrDesc = (1u << 4) | (uint32_t(kTileCols >> 3) << 17) | (uint32_t((2 * kTileRows) >> 4) << 24);
+constexpr uint32_t kInstrDesc = instr_desc_e4m3(2 * kTileRows, kTileCols);
 
 struct Shared {
     uint64_t full[kStages], empty[kStages], tmem_full[2], tmem_empty[2];
@@ -58,27 +57,6 @@ struct Shared {
 };
 constexpr size_t kSmemBytes = size_t(kStages) * kStageBytes + sizeof(Shared);
 static_assert(kSmemBytes <= 232448, "shared memory of a CTA");
-
-// Bounded wait that reads the timer only once it has polled for a while: a read takes about a microsecond, and the epilogue waits for
-// every block of 128 columns.
-__device__ __forceinline__ bool wait_block(uint64_t* bar, uint32_t parity, uint64_t limit_ns, const volatile int* abort) {
-    uint64_t start = 0;
-    uint32_t spins = 0;
-    while (!mbar_try(bar, parity)) {
-        if ((++spins & 255u) != 0u) continue;
-        if (*abort) return false;
-        const uint64_t now = timer_ns();
-        if (start == 0) start = now;
-        if (now - start > limit_ns) return false;
-    }
-    return true;
-}
-
-// Arrival without a fence: what it stands for, TMEM columns that have been read, is complete when tcgen05.wait::ld returns.  A releasing
-// arrival of cluster scope waits for the thread's loads in flight as well, the scales of the blocks ahead: 1000 cycles a block.
-__device__ __forceinline__ void arrive_read(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
 
 struct Tile {
     int expert, row0, rows, nt;  // rows: of the pair, at most 256
@@ -114,15 +92,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
                    "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                  : "r"(taddr));
 }
-__device__ __forceinline__ uint64_t pair_of(float f) {
-    uint64_t p;
-    asm("mov.b64 %0, {%1, %1};" : "=l"(p) : "r"(__float_as_uint(f)));
-    return p;
-}
-// two columns at a time: sum += {lo, hi} * f
-__device__ __forceinline__ void fma_pair(uint64_t& sum, uint32_t lo, uint32_t hi, uint64_t f) {
-    asm("{\n .reg .b64 v;\n mov.b64 v, {%1, %2};\n fma.rn.f32x2 %0, v, %3, %0;\n}" : "+l"(sum) : "r"(lo), "r"(hi), "l"(f));
-}
 template <int kRegisters>
 __device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegisters)); }
 template <int kRegisters>
@@ -157,16 +126,12 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
     }
     __syncthreads();  // the abort flag is clear before anyone sets it
     for (int e = threadIdx.x; e < args.experts; e += kThreads) {
-        const int64_t lo = args.expert_offsets != nullptr ? args.expert_offsets[e] : 0;
-        const int64_t hi = args.expert_offsets != nullptr ? args.expert_offsets[e + 1] : args.rows;
-        int64_t n = hi - lo;
-        if (lo < 0 || n < 0 || hi > args.rows || (e == 0 && lo != 0)) {
+        int64_t first, n;
+        if (!expert_range(args, e, first, n)) {
             sh.abort = 1;
             if (atomicCAS(args.status, 0u, uint32_t(kBadOffsets)) == 0u) args.status[1] = uint32_t(e);
-            n = 0;
         }
-        if (args.expert_counts != nullptr) n = max(int64_t(0), min(args.expert_counts[e], n));
-        sh.first_row[e] = int(lo);
+        sh.first_row[e] = int(first);
         sh.rows[e] = int(n);
     }
     if (warp == 1) tmem_alloc_pair(&sh.tmem_base, kTmemCols);

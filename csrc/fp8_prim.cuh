@@ -1,0 +1,63 @@
+// Device helpers shared by the 8-bit grouped GEMM kernels.
+#pragma once
+#include "fp8_gemm_sm100.hpp"
+#include "tc_prim.cuh"
+
+namespace nep {
+namespace fp8 {
+
+constexpr int kScaleBlocks = 8;  // blocks whose scales are loaded at a time: 32 bytes of a row
+
+// e4m3 x e4m3 -> fp32, both operands K-major, tile M x N
+constexpr __host__ __device__ uint32_t instr_desc_e4m3(int m, int n) { return (1u << 4) | (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24); }
+
+// Rows of an expert; false where the offsets fall, do not start at 0 or end behind the rows (it has none then).
+__device__ __forceinline__ bool expert_range(const Args& args, int e, int64_t& first, int64_t& n) {
+    first = args.expert_offsets != nullptr ? args.expert_offsets[e] : 0;
+    const int64_t end = args.expert_offsets != nullptr ? args.expert_offsets[e + 1] : args.rows;
+    n = end - first;
+    if (first < 0 || n < 0 || end > args.rows || (e == 0 && first != 0)) {
+        n = 0;
+        return false;
+    }
+    if (args.expert_counts != nullptr) n = max(int64_t(0), min(args.expert_counts[e], n));
+    return true;
+}
+
+// Bounded wait that reads the timer only once it has polled for a while: a read takes about a microsecond, and the epilogue waits for
+// every block of 128 columns.
+__device__ __forceinline__ bool wait_block(uint64_t* bar, uint32_t parity, uint64_t limit_ns, const volatile int* abort) {
+    uint64_t start = 0;
+    uint32_t spins = 0;
+    while (!gemm::tc::mbar_try(bar, parity)) {
+        if ((++spins & 255u) != 0u) continue;
+        if (*abort) return false;
+        const uint64_t now = gemm::tc::timer_ns();
+        if (start == 0) start = now;
+        if (now - start > limit_ns) return false;
+    }
+    return true;
+}
+// Arrival without a fence: what it stands for, TMEM columns that have been read, is complete when tcgen05.wait::ld returns.  A releasing
+// arrival of cluster scope waits for the thread's loads in flight as well, the scales of the blocks ahead: 1000 cycles a block.
+__device__ __forceinline__ void arrive_read(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+__device__ __forceinline__ uint64_t pair_of(float f) {
+    uint64_t p;
+    asm("mov.b64 %0, {%1, %1};" : "=l"(p) : "r"(__float_as_uint(f)));
+    return p;
+}
+__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
+    uint64_t p;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(p) : "l"(a), "l"(b));
+    return p;
+}
+// two columns at a time: sum += {lo, hi} * f
+__device__ __forceinline__ void fma_pair(uint64_t& sum, uint32_t lo, uint32_t hi, uint64_t f) {
+    asm("{\n .reg .b64 v;\n mov.b64 v, {%1, %2};\n fma.rn.f32x2 %0, v, %3, %0;\n}" : "+l"(sum) : "r"(lo), "r"(hi), "l"(f));
+}
+
+}  // namespace fp8
+}  // namespace nep

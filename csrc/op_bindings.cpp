@@ -337,10 +337,37 @@ void check_i64(const OptTensor& t, const at::Tensor& a, int64_t entries, const c
                     " must be a contiguous int64 tensor of ", std::to_string(entries), " entries on the rows' device");
 }
 
+// Which kernel an 8-bit product runs: tile = 256: rows as M, pairs of CTAs; less: weights as M, so many rows at most as N, the K axis over
+// `ctas` CTAs.  `units`: tiles that the rows allow, whatever the offsets say.
+struct Fp8Choice {
+    int64_t tile, ctas, units;
+};
+Fp8Choice choose_fp8(int64_t rows, int64_t experts, int64_t most, int64_t n_tiles, int64_t k_blocks, int64_t sms, int64_t tile, int64_t ctas) {
+    const int64_t holders = std::min(experts, rows), average = (rows + holders - 1) / holders;
+    if (experts == 1 || most <= 0 || most > rows) most = experts == 1 ? rows : rows - holders + 1;
+    Fp8Choice c{};
+    c.tile = tile > 0 ? tile : average > 192 ? 256 : most <= 32 || average <= 20 ? 32 : most <= 64 || average <= 40 ? 64 : 128;
+    c.units = (rows / c.tile + holders) * n_tiles;
+    const int64_t likely = holders * ((average + c.tile - 1) / c.tile) * n_tiles;
+    c.ctas = ctas > 0 ? ctas : 1;
+    if (ctas <= 0 && c.tile <= 128) {
+        // the split that is through first: whole passes of the clusters over the tiles, and about three blocks' time for the exchange
+        int64_t best = -1;
+        for (int64_t s = 1; s <= 8; s *= 2) {
+            const int64_t clusters = fp8::few_clusters(int(s), int(sms)), time = (likely + clusters - 1) / clusters * ((k_blocks + s - 1) / s + 3);
+            if (best < 0 || time < best) {
+                best = time;
+                c.ctas = s;
+            }
+        }
+    }
+    return c;
+}
+
 // (out) or (q, scales)
 std::vector<at::Tensor> grouped_gemm_fp8(const at::Tensor& a, const at::Tensor& a_scales, const at::Tensor& w, const at::Tensor& w_scales,
                                          const OptTensor& expert_offsets, const OptTensor& expert_counts, const OptTensor& row_scale, bool swiglu, bool quantize,
-                                         int64_t max_expert_rows, const at::Tensor& status) {
+                                         int64_t max_expert_rows, const at::Tensor& status, int64_t tile, int64_t ctas) {
     check_e4m3(a, 2, "a");
     check_e4m3(w, 3, "w");
     const int64_t rows = a.size(0), K = a.size(1), E = w.size(0), halves = swiglu ? 2 : 1;
@@ -367,6 +394,8 @@ std::vector<at::Tensor> grouped_gemm_fp8(const at::Tensor& a, const at::Tensor& 
                         row_scale->dim() == 1 && row_scale->size(0) == rows,
                     "row_scale must be contiguous float32 [rows] on the rows' device (without swiglu)");
     TORCH_CHECK(max_expert_rows >= 0, "max_expert_rows must not be negative");
+    TORCH_CHECK((tile == 0 || tile == 32 || tile == 64 || tile == 128 || tile == 256) && (ctas == 0 || ctas == 1 || ctas == 2 || ctas == 4 || ctas == 8),
+                "tile must be 0, 32, 64, 128 or 256 and ctas 0, 1, 2, 4 or 8");
     check_status_tensor(status, a);
     c10::cuda::CUDAGuard guard(a.device());
     std::vector<at::Tensor> out;
@@ -377,9 +406,6 @@ std::vector<at::Tensor> grouped_gemm_fp8(const at::Tensor& a, const at::Tensor& 
         out.push_back(at::empty({rows, n}, a.options().dtype(at::kBFloat16)));
     }
     if (rows == 0) return out;
-    fp8::Maps maps{};
-    maps.weights = e4m3_map(w.data_ptr(), K, n, E * halves, swiglu ? 64 : 128);
-    for (int b = 0; b < 4; ++b) maps.rows[b] = e4m3_map(a.data_ptr(), K, rows, 0, 128 >> b);
     fp8::Args g{};
     g.a_scales = a_scales.data_ptr<float>();
     g.w_scales = w_scales.data_ptr<float>();
@@ -401,9 +427,14 @@ std::vector<at::Tensor> grouped_gemm_fp8(const at::Tensor& a, const at::Tensor& 
     g.swiglu = swiglu;
     g.status = reinterpret_cast<uint32_t*>(status.data_ptr<int>());
     g.timeout_ns = uint64_t(5e9);
-    // a cluster for every tile that the rows allow, as far as the GPU holds them
-    const int64_t tiles = (rows / 256 + std::min(E, rows)) * g.n_tiles;
-    launched(fp8::launch(maps, g, int(std::min<int64_t>(sm_count(), 2 * tiles)), c10::cuda::getCurrentCUDAStream()), "grouped_gemm_fp8");
+    const int sms = sm_count();
+    const Fp8Choice c = choose_fp8(rows, E, max_expert_rows, g.n_tiles, g.k_blocks, sms, tile, ctas);
+    fp8::Maps maps{};
+    maps.weights = e4m3_map(w.data_ptr(), K, n, E * halves, swiglu && c.tile > 128 ? 64 : 128);
+    for (int b = 0; b < 4; ++b) maps.rows[b] = e4m3_map(a.data_ptr(), K, rows, 0, 128 >> b);
+    const auto stream = c10::cuda::getCurrentCUDAStream();
+    launched(c.tile > 128 ? fp8::launch(maps, g, int(std::min<int64_t>(sms, 2 * c.units)), stream) : fp8::launch_few(maps, g, int(c.tile), int(c.ctas), c.units, sms, stream),
+             "grouped_gemm_fp8");
     return out;
 }
 
@@ -419,7 +450,7 @@ void bind_ops(pybind11::module_& m) {
     m.def("unsort_tokens", &unsort_tokens, py::arg("y"), py::arg("slots"), py::arg("slot_map"), py::arg("weights"), py::arg("bias"));
     m.def("unsort_tokens_grad", &unsort_tokens_grad, py::arg("grad_out"), py::arg("y"), py::arg("slots"), py::arg("slot_map"), py::arg("weights"));
     m.def("grouped_gemm_fp8", &grouped_gemm_fp8, py::arg("a"), py::arg("a_scales"), py::arg("w"), py::arg("w_scales"), py::arg("expert_offsets"),
-          py::arg("expert_counts"), py::arg("row_scale"), py::arg("swiglu"), py::arg("quantize"), py::arg("max_expert_rows"), py::arg("status"));
+          py::arg("expert_counts"), py::arg("row_scale"), py::arg("swiglu"), py::arg("quantize"), py::arg("max_expert_rows"), py::arg("status"), py::arg("tile") = 0, py::arg("ctas") = 0);
 }
 
 }  // namespace nep

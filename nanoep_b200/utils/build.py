@@ -37,6 +37,7 @@ SOURCES = (
     "rms_norm.cu",
     "token_order.cu",
     "fp8_gemm_sm100.cu",
+    "fp8_gemm_few_sm100.cu",
 )
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -135,6 +135,22 @@ def test_rows_that_do_not_exist(alignment, tail, quantize):
     assert bool(same[keep].all())
 
 
+@pytest.mark.parametrize("counts", [[1], [16], [17, 0, 40], [129, 300, 0, 5], [33, 64, 65, 128, 256, 257]])
+@pytest.mark.parametrize("tile,ctas", [(32, 1), (32, 2), (32, 4), (32, 8), (64, 1), (64, 2), (64, 8), (128, 1), (128, 4), (256, 1)])
+@pytest.mark.parametrize("K,n,swiglu,quantize,scaled", [(128, 48, False, False, True), (2064, 400, False, True, False), (1024, 384, True, True, False), (400, 144, True, False, False)])
+def test_every_kernel(counts, tile, ctas, K, n, swiglu, quantize, scaled):
+    """Every tile and split of the K axis, also where a CTA's part of it is empty."""
+    a, sa, w, sw, offsets, c, real = _problem(counts, K, 2 * n if swiglu else n, swiglu=swiglu, tail=2)
+    scale = torch.rand(len(a), device="cuda") + 0.5 if scaled else None
+    got = gg._ext().grouped_gemm_fp8(a, sa, w, sw, offsets, None, scale, swiglu, quantize, 0, gg.status_tensor(a.device), tile, ctas)
+    gg.check_status()
+    want, off = _reference(a, sa, w, sw, offsets, c, swiglu, scale)
+    if quantize:
+        _check_quantized(*got, want, off, real)
+    else:
+        _check(got[0], want, off, real)
+
+
 @pytest.mark.parametrize("rows", [1, 3, 64, 129])
 def test_one_matrix(rows):
     a, sa, w, sw, offsets, n, real = _problem([rows], 768, 384)
