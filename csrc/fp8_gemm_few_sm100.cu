@@ -83,31 +83,6 @@ __device__ __forceinline__ Tile locate(const Shared<kTileRows>& sh, int experts,
     return Tile{lo, sh.first_row[lo] + start, min(each, n - start), j / tiles};
 }
 
-__device__ __forceinline__ void tma_load_2d(void* smem_dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(smem_dst)),
-                 "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y)
-                 : "memory");
-}
-__device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(smem_dst)),
-                 "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
-                 : "memory");
-}
-__device__ __forceinline__ void tmem_alloc(uint32_t* smem_slot, uint32_t cols) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_slot)), "r"(cols) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_dealloc(uint32_t addr, uint32_t cols) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
-}
-__device__ __forceinline__ void tc_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ void mma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}" ::"r"(d_tmem), "l"(a_desc),
-                 "l"(b_desc), "r"(idesc), "r"(accumulate)
-                 : "memory");
-}
 // 8 consecutive fp32 columns of this thread's TMEM lane
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t* r) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
@@ -487,8 +462,9 @@ cudaError_t launch_mode(const Maps& maps, const Args& args, int tile, int ctas, 
 
 }  // namespace
 
-// Clusters of so many CTAs that the GPU holds at a time.  Its SMs come in groups of 16 to 20 that a cluster does not leave.
-int few_clusters(int ctas, int sms) { return ctas <= 2 ? sms / ctas : sms / 20 * (20 / ctas); }
+// Clusters of so many CTAs that the GPU holds at a time (what the runtime's occupancy query answers): its SMs come in groups that a
+// cluster does not leave.  One cluster more runs behind the others and doubles the time.
+int few_clusters(int ctas, int sms) { return ctas <= 2 ? sms / ctas : ctas == 4 ? 33 * sms / 148 : 15 * sms / 148; }
 
 cudaError_t launch_few(const Maps& maps, const Args& args, int tile, int ctas, int64_t units, int sms, cudaStream_t stream) {
     if (args.experts > kMaxExperts || units < 1 || ctas < 1 || ctas > 8) return cudaErrorInvalidValue;

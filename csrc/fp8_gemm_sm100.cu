@@ -29,62 +29,66 @@ namespace {
 using namespace gemm::tc;
 using namespace rows;
 
-constexpr int kTileRows = 128;                   // of one CTA
-constexpr int kTileCols = 256;                   // weight rows of a pair
-constexpr int kHalfBytes = 128 * 128;            // 16 KB: this CTA's rows, or its half of the weight rows
-constexpr int kStageBytes = 2 * kHalfBytes;
-constexpr int kStages = 6;
+constexpr int kTileRows = 128;
+constexpr int kTileCols = 256;                   // weight rows
+constexpr int kRowBytes = kTileRows * 128, kWeightBytes = kTileCols * 128;
+constexpr int kStageBytes = kRowBytes + kWeightBytes;
+constexpr int kStages = 4;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 128 + 32 * kEpiWarps;   // a warpgroup that loads and issues, two that add up
-// A launch of 384 threads gives each 168 registers.  The sums need more: 80 + 2 * 208 < 3 * 168, what the block was launched with.
-constexpr int kFewRegisters = 80, kManyRegisters = 208;
+// A launch of 384 threads gives each 168 registers.  The sums need more: 72 + 2 * 208 < 3 * 168, what the block was launched with.
+constexpr int kFewRegisters = 72, kManyRegisters = 208;
 static_assert(128 * kFewRegisters + 32 * kEpiWarps * kManyRegisters <= kThreads * 168, "registers of the launch");
 constexpr int kTmemCols = 512;
-constexpr uint32_t kInstrDesc = instr_desc_e4m3(2 * kTileRows, kTileCols);
+constexpr int kPieceBytes = 64, kPiecePitch = kPieceBytes + 16;  // of an output row on its way out: 8 rows hit all banks once
+constexpr uint32_t kInstrDesc = instr_desc_e4m3(kTileRows, kTileCols);
 
 struct Shared {
-    uint64_t full[kStages], empty[kStages], tmem_full[2], tmem_empty[2];
+    uint8_t piece[kEpiWarps][32 * kPiecePitch];
+    float row_scales[2][kScaleBlocks][kTileRows];  // of the next blocks, by turns
+    float weight_scales[2][kScaleBlocks][2];       // of the tile's two halves (of the gate and up rows)
+    float most[2][2][kTileRows];                   // largest of each row's 64 columns, by parity of the tile and epilogue group
+    uint64_t full[kStages], done[kStages], tmem_empty[2];
     uint64_t scale_full[2], scale_empty[2];
-    uint64_t told[2][4];               // by epilogue group and quarter: its rows' largest values are in `most`
+    uint64_t told[2][4];                           // by epilogue group and quarter: its rows' largest values are in `most`
     uint32_t tmem_base;
     int abort;
-    float row_scales[2][kScaleBlocks][kTileRows];  // of the next blocks, by turns
-    float weight_scales[2][kScaleBlocks][2];       // of the pair's two halves (of the gate and up rows)
-    float most[2][2][kTileRows];       // largest of each row's 64 columns, by parity of the tile and epilogue group
-    int first_row[kMaxExperts];
-    int rows[kMaxExperts];
-    int first_tile[kMaxExperts + 1];   // exclusive prefix of row tiles
+    int first_tile[kMaxExperts + 1];               // exclusive prefix of row tiles
 };
 constexpr size_t kSmemBytes = size_t(kStages) * kStageBytes + sizeof(Shared);
 static_assert(kSmemBytes <= 232448, "shared memory of a CTA");
 
 struct Tile {
-    int expert, row0, rows, nt;  // rows: of the pair, at most 256
+    int expert, row0, rows, nt;
 };
 // The row tiles that share a weight tile are neighbours: the weights come from memory once and from L2 afterwards.
-__device__ __forceinline__ Tile locate(const Shared& sh, int experts, int n_tiles, int unit) {
-    const int at = unit / n_tiles;
-    int lo = 0, hi = experts;  // first_tile[lo] <= at < first_tile[hi]
+__device__ __forceinline__ Tile tile_of(const Shared& sh, const Args& args, int unit, int expert) {
+    const int tiles = sh.first_tile[expert + 1] - sh.first_tile[expert], j = unit - sh.first_tile[expert] * args.n_tiles;
+    int64_t first, n;
+    expert_range(args, expert, first, n);
+    const int start = j % tiles * kTileRows;
+    return Tile{expert, int(first) + start, min(kTileRows, int(n) - start), j / tiles};
+}
+__device__ __forceinline__ Tile locate(const Shared& sh, const Args& args, int unit) {
+    const int at = unit / args.n_tiles;
+    int lo = 0, hi = args.experts;  // first_tile[lo] <= at < first_tile[hi]
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (sh.first_tile[mid] <= at) lo = mid; else hi = mid;
     }
-    const int tiles = sh.first_tile[lo + 1] - sh.first_tile[lo], j = unit - sh.first_tile[lo] * n_tiles;
-    const int start = j % tiles * 2 * kTileRows;
-    return Tile{lo, sh.first_row[lo] + start, min(2 * kTileRows, sh.rows[lo] - start), j / tiles};
+    return tile_of(sh, args, unit, lo);
+}
+// The same by a whole warp: 32 places at a look.
+__device__ __forceinline__ Tile locate_warp(const Shared& sh, const Args& args, int unit, int lane) {
+    const int at = unit / args.n_tiles;
+    int lo = 0;
+    for (int step = args.experts > 32 ? 32 : 1; step >= 1; step /= 32) {
+        const int e = lo + lane * step;
+        lo += step * (__popc(__ballot_sync(0xffffffffu, e < args.experts && sh.first_tile[e] <= at)) - 1);
+    }
+    return tile_of(sh, args, unit, lo);
 }
 
-__device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar_cluster_addr) {
-    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
-                     smem_u32(smem_dst)),
-                 "l"(map), "r"(bar_cluster_addr), "r"(x), "r"(y), "r"(z)
-                 : "memory");
-}
-__device__ __forceinline__ void mma_pair_e4m3(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t accumulate) {
-    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}" ::"r"(d_tmem),
-                 "l"(a_desc), "l"(b_desc), "r"(kInstrDesc), "r"(accumulate)
-                 : "memory");
-}
 // 16 consecutive fp32 columns of this thread's TMEM lane
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
@@ -92,6 +96,13 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
                    "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                  : "r"(taddr));
 }
+// A row's piece leaves by a copy of its thread's own: whole sectors, and nothing waits for them but the piece's next use.
+__device__ __forceinline__ void send_piece(void* dst, const void* piece, int bytes) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(piece)), "r"(bytes) : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void pieces_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 template <int kRegisters>
 __device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegisters)); }
 template <int kRegisters>
@@ -102,20 +113,15 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
     extern __shared__ __align__(1024) uint8_t smem[];
     Shared& sh = *reinterpret_cast<Shared*>(smem + kStages * kStageBytes);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t cta = cluster_ctarank();
-    const bool leader = cta == 0;
     const uint64_t limit_ns = args.timeout_ns;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
-            mbar_init(&sh.full[s], 1);   // leader: one expect_tx arrival covering both CTAs' bytes
-            mbar_init(&sh.empty[s], 1);  // one commit from the leader's MMA thread
+            mbar_init(&sh.full[s], 1);
+            mbar_init(&sh.done[s], 1);  // one commit: the stage is free and its block sums are in TMEM
         }
         for (int b = 0; b < 2; ++b) {
-            mbar_init(&sh.tmem_full[b], 1);
-            mbar_init(&sh.tmem_empty[b], 2 * kEpiWarps);  // leader: the epilogue warps of both CTAs
-        }
-        for (int b = 0; b < 2; ++b) {
+            mbar_init(&sh.tmem_empty[b], kEpiWarps);
             mbar_init(&sh.scale_full[b], 1);
             mbar_init(&sh.scale_empty[b], kEpiWarps);
         }
@@ -131,16 +137,15 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
             sh.abort = 1;
             if (atomicCAS(args.status, 0u, uint32_t(kBadOffsets)) == 0u) args.status[1] = uint32_t(e);
         }
-        sh.first_row[e] = int(first);
-        sh.rows[e] = int(n);
+        sh.first_tile[e] = int((n + kTileRows - 1) / kTileRows);
     }
-    if (warp == 1) tmem_alloc_pair(&sh.tmem_base, kTmemCols);
+    if (warp == 1) tmem_alloc(&sh.tmem_base, kTmemCols);
     __syncthreads();
     if (warp == 0) {
         int carry = 0;
         for (int base = 0; base < args.experts; base += 32) {
             const int e = base + lane;
-            const int tiles = e < args.experts && !sh.abort ? (sh.rows[e] + 2 * kTileRows - 1) / (2 * kTileRows) : 0;
+            const int tiles = e < args.experts && !sh.abort ? sh.first_tile[e] : 0;
             int incl = tiles;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
@@ -154,12 +159,10 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
     }
     tc_fence_before();
     __syncthreads();
-    cluster_sync();  // both CTAs have initialised their barriers before anyone signals across
     tc_fence_after();
     const uint32_t tmem_base = sh.tmem_base;
 
     const int k_blocks = args.k_blocks;
-    const int cluster_id = blockIdx.x >> 1, num_clusters = gridDim.x >> 1;
     const int units = sh.first_tile[args.experts] * args.n_tiles;  // none after bad offsets
     volatile int* abort_flag = &sh.abort;
     auto fail = [&](uint32_t code) {
@@ -170,37 +173,37 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
     if (warp < 4) {
     give_registers<kFewRegisters>();
     if (warp == 0) {
-        // ------------------------------------------------------------------ TMA producer (both CTAs)
+        // ------------------------------------------------------------------ TMA producer
         if (elect_one()) {
             int stage = 0;
             uint32_t phase = 0;
             int64_t issued = 0;
-            for (int unit = cluster_id; unit < units && !*abort_flag; unit += num_clusters) {
-                const Tile t = locate(sh, args.experts, args.n_tiles, unit);
+            for (int unit = int(blockIdx.x); unit < units && !*abort_flag; unit += int(gridDim.x)) {
+                const Tile t = locate(sh, args, unit);
                 // rows that exist, in 16s; what the others' places hold reaches only their own sums
-                const int both = (t.rows + 15) & ~15, mine = max(0, min(kTileRows, both - int(cta) * kTileRows));
-                const uint32_t bytes = uint32_t(2 * kHalfBytes + both * 128);
+                const int n = (t.rows + 15) & ~15;
                 for (int kb = 0; kb < k_blocks; ++kb) {
-                    if (!wait_block(&sh.empty[stage], phase ^ 1u, limit_ns, abort_flag)) {
+                    if (!wait_block(&sh.done[stage], phase ^ 1u, limit_ns, abort_flag)) {
                         fail(kPipeTimeout);
                         break;
                     }
-                    uint8_t* dst = smem + stage * kStageBytes;
-                    const uint32_t bar = map_to_cta(smem_u32(&sh.full[stage]), 0);
-                    if (leader) mbar_expect_tx(&sh.full[stage], bytes);
-                    if (kSwiGLU) {
-                        const int f0 = t.nt * 128 + int(cta) * 64;
-                        tma_load_3d_pair(dst + kHalfBytes, &maps.weights, kb * 128, f0, 2 * t.expert, bar);
-                        tma_load_3d_pair(dst + kHalfBytes + kHalfBytes / 2, &maps.weights, kb * 128, f0, 2 * t.expert + 1, bar);
+                    uint8_t *dst = smem + stage * kStageBytes, *w_dst = dst + kRowBytes;
+                    mbar_expect_tx(&sh.full[stage], uint32_t(kWeightBytes + n * 128));
+                    if (kSwiGLU) {  // 64 gate rows, their 64 up rows, and again
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            tma_load_3d(w_dst + q * 64 * 128, &maps.weights, kb * 128, t.nt * 128 + (q >> 1) * 64, 2 * t.expert + (q & 1), &sh.full[stage]);
                     } else {
-                        tma_load_3d_pair(dst + kHalfBytes, &maps.weights, kb * 128, t.nt * kTileCols + int(cta) * 128, t.expert, bar);
+#pragma unroll
+                        for (int q = 0; q < 2; ++q)
+                            tma_load_3d(w_dst + q * 128 * 128, &maps.weights, kb * 128, t.nt * kTileCols + q * 128, t.expert, &sh.full[stage]);
                     }
                     int at = 0;  // boxes of 128, 64, 32 and 16 rows make up any multiple of 16
 #pragma unroll
                     for (int b = 0; b < 4; ++b) {
                         const int box = 128 >> b;
-                        if (mine & box) {
-                            tma_load_2d_pair(dst + at * 128, &maps.rows[b], kb * 128, t.row0 + int(cta) * kTileRows + at, bar);
+                        if (n & box) {
+                            tma_load_2d(dst + at * 128, &maps.rows[b], kb * 128, t.row0 + at, &sh.full[stage]);
                             at += box;
                         }
                     }
@@ -211,21 +214,16 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                     }
                 }
             }
-            // a kernel that gave up does not end under its own copies (the leader's barriers count those of both CTAs)
-            if (*abort_flag && leader)
+            if (*abort_flag)  // a kernel that gave up does not end under its own copies
                 for (int64_t i = max(int64_t(0), issued - kStages); i < issued; ++i)
                     mbar_wait(&sh.full[i % kStages], uint32_t(i / kStages) & 1u, min(limit_ns, uint64_t(100000000)));
         }
     } else if (warp == 1) {
-        // ------------------------------------------------------------------ MMA issuer (leader CTA only)
-        if (leader && elect_one()) {
+        // ------------------------------------------------------------------ MMA issuer
+        if (elect_one()) {
             int stage = 0, block = 0;
             uint32_t phase = 0;
-            auto commit = [&](uint64_t* bar) {  // in both CTAs, once the MMAs so far have been done
-                tc_commit_pair(map_to_cta(smem_u32(bar), 0));
-                tc_commit_pair(map_to_cta(smem_u32(bar), 1));
-            };
-            for (int unit = cluster_id; unit < units && !*abort_flag; unit += num_clusters) {
+            for (int unit = int(blockIdx.x); unit < units && !*abort_flag; unit += int(gridDim.x)) {
                 for (int kb = 0; kb < k_blocks; ++kb, ++block) {
                     const int buf = block & 1;
                     if (!wait_block(&sh.full[stage], phase, limit_ns, abort_flag) || !wait_block(&sh.tmem_empty[buf], (uint32_t(block >> 1) & 1u) ^ 1u, limit_ns, abort_flag)) {
@@ -234,12 +232,13 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                     }
                     tc_fence_after();
                     const uint8_t* tile = smem + stage * kStageBytes;
-                    const uint64_t a_desc = smem_desc_sw128(tile), b_desc = smem_desc_sw128(tile + kHalfBytes);
+                    const uint64_t a_desc = smem_desc_sw128(tile), b_desc = smem_desc_sw128(tile + kRowBytes);
 #pragma unroll
                     for (int k = 0; k < 4; ++k)  // 32 values = 32 bytes inside the 128-byte swizzle row
-                        mma_pair_e4m3(tmem_base + uint32_t(buf * kTileCols), a_desc + uint64_t(k * 2), b_desc + uint64_t(k * 2), k != 0 ? 1u : 0u);
-                    commit(&sh.empty[stage]);
-                    commit(&sh.tmem_full[buf]);
+                        mma_e4m3(tmem_base + uint32_t(buf * kTileCols), a_desc + uint64_t(k * 2), b_desc + uint64_t(k * 2), kInstrDesc, k != 0 ? 1u : 0u);
+                    // One barrier per stage tells both the producer and the epilogue.  The epilogue has seen a block before the stage's next one can
+                    // be done: that one waits for its TMEM columns.
+                    tc_commit(&sh.done[stage]);
                     if (++stage == kStages) {
                         stage = 0;
                         phase ^= 1u;
@@ -248,41 +247,40 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
             }
         }
     } else if (warp == 2) {
-        // ------------------------------------------------------------------ scales (both CTAs)
+        // ------------------------------------------------------------------ scales
         // Eight blocks at a time and up to sixteen ahead: the epilogue warps have no registers left to wait for memory.
         constexpr int kHalves = kSwiGLU ? 2 : 1;
         int chunk = 0;
         bool ok = true;
-        for (int unit = cluster_id; unit < units && ok; unit += num_clusters) {
-            const Tile t = locate(sh, args.experts, args.n_tiles, unit);
+        for (int unit = int(blockIdx.x); unit < units && ok; unit += int(gridDim.x)) {
+            const Tile t = locate_warp(sh, args, unit, lane);
             // 128 weight rows share a scale: the two halves of the tile, or those of its gate and up rows
             const int half = lane & 1, block = kSwiGLU ? half * args.n_blocks + t.nt : min(2 * t.nt + half, args.n_blocks - 1);
             const float* sw = args.w_scales + (int64_t(t.expert) * kHalves * args.n_blocks + block) * k_blocks;
-            const float* sa[4];
-            bool real[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = int(cta) * kTileRows + i * 32 + lane;
-                real[i] = r < t.rows;
-                sa[i] = args.a_scales + (int64_t(t.row0) + r) * k_blocks;
-            }
             for (int kb0 = 0; kb0 < k_blocks; kb0 += kScaleBlocks, ++chunk) {
-                float v[4][kScaleBlocks];
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < kScaleBlocks; ++j) v[i][j] = real[i] && kb0 + j < k_blocks ? sa[i][kb0 + j] : 0.f;
                 const float w = kb0 + (lane >> 1) < k_blocks && lane < 2 * kScaleBlocks ? sw[kb0 + (lane >> 1)] : 0.f;
                 const int slot = chunk & 1;
-                ok = __all_sync(0xffffffffu, wait_block(&sh.scale_empty[slot], (uint32_t(chunk >> 1) & 1u) ^ 1u, limit_ns, abort_flag));
+#pragma unroll
+                for (int i = 0; i < 4; i += 2) {  // two rows a lane at a time, for want of registers
+                    float v[2][kScaleBlocks];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int r = (i + h) * 32 + lane;
+                        const float* sa = args.a_scales + (int64_t(t.row0) + r) * k_blocks + kb0;
+#pragma unroll
+                        for (int j = 0; j < kScaleBlocks; ++j) v[h][j] = r < t.rows && kb0 + j < k_blocks ? sa[j] : 0.f;
+                    }
+                    if (i == 0) ok = __all_sync(0xffffffffu, wait_block(&sh.scale_empty[slot], (uint32_t(chunk >> 1) & 1u) ^ 1u, limit_ns, abort_flag));
+                    if (!ok) break;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int j = 0; j < kScaleBlocks; ++j) sh.row_scales[slot][j][(i + h) * 32 + lane] = v[h][j];
+                }
                 if (!ok) {
                     if (lane == 0) fail(kPipeTimeout);
                     break;
                 }
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < kScaleBlocks; ++j) sh.row_scales[slot][j][i * 32 + lane] = v[i][j];
                 if (lane < 2 * kScaleBlocks) sh.weight_scales[slot][lane >> 1][half] = w;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.scale_full[slot]);
@@ -290,70 +288,111 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
         }
     }
     } else {
-        // ------------------------------------------------------------------ epilogue (both CTAs)
+        // ------------------------------------------------------------------ epilogue
         take_registers<kManyRegisters>();
         const int quarter = warp & 3;        // TMEM lanes [32 * quarter, +32) belong to this warp
         const int group = (warp - 4) >> 2;   // its 128 columns
         const int r = quarter * 32 + lane;   // row of this CTA's tile
-        int block = 0, chunk = 0, exchanges = 0;
+        const uint32_t empty_addr = smem_u32(&sh.tmem_empty[0]);
+        uint8_t* piece = sh.piece[warp - 4] + lane * kPiecePitch;  // this thread's row
+        int block = 0, stage = 0, chunk = 0, exchanges = 0;
+        uint32_t phase = 0;
         bool ok = true;
-        for (int unit = cluster_id; unit < units && ok; unit += num_clusters) {
-            const Tile t = locate(sh, args.experts, args.n_tiles, unit);
-            const int in_tile = int(cta) * kTileRows + r;
-            const bool real = in_tile < t.rows;
-            const bool any = int(cta) * kTileRows + quarter * 32 < t.rows;  // of this warp's rows
-            const int64_t row = int64_t(t.row0) + in_tile;
+        for (int unit = int(blockIdx.x); unit < units && ok; unit += int(gridDim.x)) {
+            const Tile t = locate_warp(sh, args, unit, lane);
+            const bool real = r < t.rows;
+            const bool any = quarter * 32 < t.rows;  // of this warp's rows
+            const int64_t row = int64_t(t.row0) + r;
             const int wb = kSwiGLU ? t.nt : t.nt * 2 + group;  // output block of this thread
             const bool inside = wb < args.n_blocks;
             uint64_t sum[64];  // pairs of neighbouring columns
 #pragma unroll
             for (int j = 0; j < 64; ++j) sum[j] = 0;
+            // Under the MMAs' operand traffic an access to shared memory takes 200 to 300 cycles, a look at a barrier as well: scales and the state of
+            // the next block are asked for while a block is added, and used behind it.
+            float sr = 0.f, sw0 = 0.f, sw1 = 0.f, f0 = 0.f, f1 = 0.f;
+            auto fetch_scales = [&](int kb) {
+                const int at = kb % kScaleBlocks, slot = chunk & 1;
+                if (at == 0) ok = __all_sync(0xffffffffu, wait_block(&sh.scale_full[slot], uint32_t(chunk >> 1) & 1u, limit_ns, abort_flag)) && ok;
+                sr = sh.row_scales[slot][at][r];
+                sw0 = sh.weight_scales[slot][at][kSwiGLU ? 0 : group];
+                if (kSwiGLU) sw1 = sh.weight_scales[slot][at][1];
+            };
+            auto use_scales = [&](int kb) {
+                f0 = sr * sw0;
+                if (kSwiGLU) f1 = sr * sw1;
+                if (kb % kScaleBlocks == kScaleBlocks - 1 || kb == k_blocks - 1) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.scale_empty[chunk & 1]);
+                    ++chunk;
+                }
+            };
+            // A block is 16, 32, 16, 32, 16 and 16 columns, the next ones on their way while these are added; the first of a block under the last
+            // of the one before, where it is complete by then.  (One after the other a block took 1070 cycles, mostly latencies.)
+            const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(group * 128);
+            uint32_t a[32], b[16];
+            fetch_scales(0);
+            use_scales(0);
+            bool begun = false;  // the loads of the block's first columns have been issued
             for (int kb = 0; kb < k_blocks; ++kb, ++block) {
                 const int buf = block & 1;
-                const int at = kb % kScaleBlocks, slot = chunk & 1;
-                if (at == 0) {
-                    ok = __all_sync(0xffffffffu, wait_block(&sh.scale_full[slot], uint32_t(chunk >> 1) & 1u, limit_ns, abort_flag));
+                if (!begun) {
+                    ok = __all_sync(0xffffffffu, wait_block(&sh.done[stage], phase, limit_ns, abort_flag)) && ok;
                     if (!ok) {
                         if (lane == 0) fail(kPipeTimeout);
                         break;
                     }
+                    tc_fence_after();
+                    if (any) tmem_ld16(taddr + uint32_t(buf * kTileCols), b);
                 }
-                const float s = sh.row_scales[slot][at][r];
-                const uint64_t f0 = pair_of(s * sh.weight_scales[slot][at][kSwiGLU ? 0 : group]);
-                const uint64_t f1 = kSwiGLU ? pair_of(s * sh.weight_scales[slot][at][1]) : f0;
-                if (at == kScaleBlocks - 1 || kb == k_blocks - 1) {
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sh.scale_empty[slot]);
-                    ++chunk;
+                if (++stage == kStages) {
+                    stage = 0;
+                    phase ^= 1u;
                 }
-                ok = __all_sync(0xffffffffu, wait_block(&sh.tmem_full[buf], uint32_t(block >> 1) & 1u, limit_ns, abort_flag));
-                if (!ok) {
-                    if (lane == 0) fail(kPipeTimeout);
-                    break;
-                }
-                tc_fence_after();
-                auto drained = [&]() {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) arrive_read(map_to_cta(smem_u32(&sh.tmem_empty[buf]), 0));
-                };
                 if (any) {
-                    // the next 16 columns are on their way while these are added
-                    const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(buf * kTileCols + group * 128);
-                    uint32_t v[2][16];
-                    tmem_ld16(taddr, v[0]);
+                    const uint32_t at = taddr + uint32_t(buf * kTileCols);
+                    const uint64_t g0 = pair_of(f0), g1 = kSwiGLU ? pair_of(f1) : g0;
+                    auto add_a = [&](int c, int pairs) {
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) {
-                        tmem_ld_wait();
-                        if (c < 7) tmem_ld16(taddr + (c + 1) * 16, v[(c + 1) & 1]);
-                        else drained();
-                        const uint64_t f = c < 4 ? f0 : f1;
+                        for (int j = 0; j < 16; ++j)
+                            if (j < pairs) fma_pair(sum[c / 2 + j], a[2 * j], a[2 * j + 1], c < 64 ? g0 : g1);
+                    };
+                    auto add_b = [&](int c) {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) fma_pair(sum[c * 8 + j], v[c & 1][2 * j], v[c & 1][2 * j + 1], f);
+                        for (int j = 0; j < 8; ++j) fma_pair(sum[c / 2 + j], b[2 * j], b[2 * j + 1], c < 64 ? g0 : g1);
+                    };
+                    tmem_ld_wait();
+                    tmem_ld32(at + 16, a);
+                    if (kb + 1 < k_blocks) fetch_scales(kb + 1);
+                    add_b(0);
+                    tmem_ld_wait();
+                    tmem_ld16(at + 48, b);
+                    add_a(16, 16);
+                    tmem_ld_wait();
+                    tmem_ld32(at + 64, a);
+                    add_b(48);
+                    tmem_ld_wait();
+                    tmem_ld16(at + 96, b);
+                    const bool next_done = block_done(&sh.done[stage], phase);
+                    add_a(64, 16);
+                    tmem_ld_wait();
+                    tmem_ld16(at + 112, a);
+                    add_b(96);
+                    tmem_ld_wait();
+                    tc_fence_before();
+                    if (lane == 0) arrive_read(empty_addr + uint32_t(buf) * 8u);
+                    begun = __all_sync(0xffffffffu, kb + 1 < k_blocks && next_done);
+                    if (begun) {
+                        tc_fence_after();
+                        tmem_ld16(taddr + uint32_t((buf ^ 1) * kTileCols), b);
                     }
+                    add_a(112, 8);
                 } else {
-                    drained();
+                    tc_fence_before();
+                    if (lane == 0) arrive_read(empty_addr + uint32_t(buf) * 8u);
+                    if (kb + 1 < k_blocks) fetch_scales(kb + 1);
                 }
+                if (kb + 1 < k_blocks) use_scales(kb + 1);
             }
             if (!ok) break;
             if (!any) continue;
@@ -396,30 +435,40 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                 const float per = __fdiv_rn(kLargest, m);  // sums do not lie on the border of two e4m3 values: a product will do
                 if (real && (kSwiGLU ? group == 0 : inside)) args.scales[row * args.n_blocks + wb] = __fdiv_rn(m, kLargest);
 #pragma unroll
-                for (int j = 0; j < kCols; j += 16) {
-                    if (!real || n0 + j >= args.n) continue;
-                    uint32_t q[4];
+                for (int j = 0; j < kCols; j += 64) {
+                    pieces_read();
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        q[i] = pack_e4m3(acc[j + 4 * i] * per, acc[j + 4 * i + 1] * per, acc[j + 4 * i + 2] * per, acc[j + 4 * i + 3] * per);
-                    st_v4(args.q + row * args.n + n0 + j, q[0], q[1], q[2], q[3]);
+                    for (int i = 0; i < 64; i += 16) {
+                        uint32_t q[4];
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) {
+                            const float* f = acc + j + i + 4 * h;
+                            q[h] = pack_e4m3(f[0] * per, f[1] * per, f[2] * per, f[3] * per);
+                        }
+                        *reinterpret_cast<uint4*>(piece + i) = make_uint4(q[0], q[1], q[2], q[3]);
+                    }
+                    if (real && n0 + j < args.n) send_piece(args.q + row * args.n + n0 + j, piece, min(64, args.n - n0 - j));
                 }
             } else {
 #pragma unroll
-                for (int j = 0; j < kCols; j += 8) {
-                    if (!real || n0 + j >= args.n) continue;
-                    st_v4(args.out + row * args.n + n0 + j, pack_bf16(acc[j], acc[j + 1]), pack_bf16(acc[j + 2], acc[j + 3]), pack_bf16(acc[j + 4], acc[j + 5]),
-                          pack_bf16(acc[j + 6], acc[j + 7]));
+                for (int j = 0; j < kCols; j += 32) {
+                    pieces_read();
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        const float* f = acc + j + i;
+                        *reinterpret_cast<uint4*>(piece + i * 2) = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+                    }
+                    if (real && n0 + j < args.n) send_piece(args.out + row * args.n + n0 + j, piece, 2 * min(32, args.n - n0 - j));
                 }
             }
         }
+        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // the rows have left shared memory and are written
     }
     tc_fence_before();
     __syncthreads();
-    cluster_sync();  // the peer may still be reading this CTA's operands / signalling its barriers
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc_pair(tmem_base, kTmemCols);
+        tmem_dealloc(tmem_base, kTmemCols);
     }
 }
 
@@ -433,21 +482,13 @@ cudaError_t launch_mode(const Maps& maps, const Args& args, int grid, cudaStream
     config.blockDim = dim3(kThreads);
     config.dynamicSmemBytes = kSmemBytes;
     config.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    config.attrs = attr;
-    config.numAttrs = 1;
     return cudaLaunchKernelEx(&config, fn, maps, args);
 }
 
 }  // namespace
 
 cudaError_t launch(const Maps& maps, const Args& args, int grid, cudaStream_t stream) {
-    grid &= ~1;
-    if (args.experts > kMaxExperts || grid < 2) return cudaErrorInvalidValue;
+    if (args.experts > kMaxExperts || grid < 1) return cudaErrorInvalidValue;
     if (args.swiglu) return args.q != nullptr ? launch_mode<true, true>(maps, args, grid, stream) : launch_mode<true, false>(maps, args, grid, stream);
     return args.q != nullptr ? launch_mode<false, true>(maps, args, grid, stream) : launch_mode<false, false>(maps, args, grid, stream);
 }

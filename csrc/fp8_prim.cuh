@@ -24,6 +24,15 @@ __device__ __forceinline__ bool expert_range(const Args& args, int e, int64_t& f
     return true;
 }
 
+// Whether a phase is complete, without waiting: asked ahead, so that the answer's way (about 100 cycles) lies under other work.
+__device__ __forceinline__ bool block_done(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(done)
+                 : "r"(gemm::tc::smem_u32(bar)), "r"(parity)
+                 : "memory");
+    return done != 0;
+}
 // Bounded wait that reads the timer only once it has polled for a while: a read takes about a microsecond, and the epilogue waits for
 // every block of 128 columns.
 __device__ __forceinline__ bool wait_block(uint64_t* bar, uint32_t parity, uint64_t limit_ns, const volatile int* abort) {
@@ -42,6 +51,32 @@ __device__ __forceinline__ bool wait_block(uint64_t* bar, uint32_t parity, uint6
 // arrival of cluster scope waits for the thread's loads in flight as well, the scales of the blocks ahead: 1000 cycles a block.
 __device__ __forceinline__ void arrive_read(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+__device__ __forceinline__ void tma_load_2d(void* smem_dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(gemm::tc::smem_u32(smem_dst)),
+                 "l"(map), "r"(gemm::tc::smem_u32(bar)), "r"(x), "r"(y)
+                 : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(gemm::tc::smem_u32(smem_dst)),
+                 "l"(map), "r"(gemm::tc::smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_alloc(uint32_t* smem_slot, uint32_t cols) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(gemm::tc::smem_u32(smem_slot)), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc(uint32_t addr, uint32_t cols) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+}
+__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(gemm::tc::smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void mma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}" ::"r"(d_tmem), "l"(a_desc),
+                 "l"(b_desc), "r"(idesc), "r"(accumulate)
+                 : "memory");
 }
 
 __device__ __forceinline__ uint64_t pair_of(float f) {

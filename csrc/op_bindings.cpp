@@ -347,7 +347,7 @@ Fp8Choice choose_fp8(int64_t rows, int64_t experts, int64_t most, int64_t n_tile
     if (experts == 1 || most <= 0 || most > rows) most = experts == 1 ? rows : rows - holders + 1;
     Fp8Choice c{};
     c.tile = tile > 0 ? tile : average > 192 ? 256 : most <= 32 || average <= 20 ? 32 : most <= 64 || average <= 40 ? 64 : 128;
-    c.units = (rows / c.tile + holders) * n_tiles;
+    c.units = (rows / std::min<int64_t>(c.tile, 128) + holders) * n_tiles;
     const int64_t likely = holders * ((average + c.tile - 1) / c.tile) * n_tiles;
     c.ctas = ctas > 0 ? ctas : 1;
     if (ctas <= 0 && c.tile <= 128) {
@@ -433,7 +433,7 @@ std::vector<at::Tensor> grouped_gemm_fp8(const at::Tensor& a, const at::Tensor& 
     maps.weights = e4m3_map(w.data_ptr(), K, n, E * halves, swiglu && c.tile > 128 ? 64 : 128);
     for (int b = 0; b < 4; ++b) maps.rows[b] = e4m3_map(a.data_ptr(), K, rows, 0, 128 >> b);
     const auto stream = c10::cuda::getCurrentCUDAStream();
-    launched(c.tile > 128 ? fp8::launch(maps, g, int(std::min<int64_t>(sms, 2 * c.units)), stream) : fp8::launch_few(maps, g, int(c.tile), int(c.ctas), c.units, sms, stream),
+    launched(c.tile > 128 ? fp8::launch(maps, g, int(std::min<int64_t>(sms, c.units)), stream) : fp8::launch_few(maps, g, int(c.tile), int(c.ctas), c.units, sms, stream),
              "grouped_gemm_fp8");
     return out;
 }
