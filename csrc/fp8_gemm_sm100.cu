@@ -33,18 +33,19 @@ constexpr int kTileRows = 128;
 constexpr int kTileCols = 256;                   // weight rows
 constexpr int kRowBytes = kTileRows * 128, kWeightBytes = kTileCols * 128;
 constexpr int kStageBytes = kRowBytes + kWeightBytes;
-constexpr int kStages = 4;
+constexpr int kStages = 3;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 128 + 32 * kEpiWarps;   // a warpgroup that loads and issues, two that add up
 // A launch of 384 threads gives each 168 registers.  The sums need more: 72 + 2 * 208 < 3 * 168, what the block was launched with.
 constexpr int kFewRegisters = 72, kManyRegisters = 208;
 static_assert(128 * kFewRegisters + 32 * kEpiWarps * kManyRegisters <= kThreads * 168, "registers of the launch");
 constexpr int kTmemCols = 512;
-constexpr int kPieceBytes = 64, kPiecePitch = kPieceBytes + 16;  // of an output row on its way out: 8 rows hit all banks once
+constexpr int kPiecePitch = 256 + 16;            // a thread's part of an output row on its way out: 8 rows hit all banks once
 constexpr uint32_t kInstrDesc = instr_desc_e4m3(kTileRows, kTileCols);
 
 struct Shared {
-    uint8_t piece[kEpiWarps][32 * kPiecePitch];
+    alignas(16) uint8_t piece[kEpiWarps][32 * kPiecePitch];
+    int4 tile[2];                                  // of the chunk's blocks: expert, first row, rows, weight tile
     float row_scales[2][kScaleBlocks][kTileRows];  // of the next blocks, by turns
     float weight_scales[2][kScaleBlocks][2];       // of the tile's two halves (of the gate and up rows)
     float most[2][2][kTileRows];                   // largest of each row's 64 columns, by parity of the tile and epilogue group
@@ -282,6 +283,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                     break;
                 }
                 if (lane < 2 * kScaleBlocks) sh.weight_scales[slot][lane >> 1][half] = w;
+                if (lane == 0) sh.tile[slot] = make_int4(t.expert, t.row0, t.rows, t.nt);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.scale_full[slot]);
             }
@@ -299,15 +301,22 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
         uint32_t phase = 0;
         bool ok = true;
         for (int unit = int(blockIdx.x); unit < units && ok; unit += int(gridDim.x)) {
-            const Tile t = locate_warp(sh, args, unit, lane);
+            // the warp that loads the scales knows the tile already
+            ok = __all_sync(0xffffffffu, wait_block(&sh.scale_full[chunk & 1], uint32_t(chunk >> 1) & 1u, limit_ns, abort_flag));
+            if (!ok) {
+                if (lane == 0) fail(kPipeTimeout);
+                break;
+            }
+            const int4 told = sh.tile[chunk & 1];
+            const Tile t{told.x, told.y, told.z, told.w};
             const bool real = r < t.rows;
             const bool any = quarter * 32 < t.rows;  // of this warp's rows
             const int64_t row = int64_t(t.row0) + r;
             const int wb = kSwiGLU ? t.nt : t.nt * 2 + group;  // output block of this thread
             const bool inside = wb < args.n_blocks;
-            uint64_t sum[64];  // pairs of neighbouring columns
+            float acc[128];
 #pragma unroll
-            for (int j = 0; j < 64; ++j) sum[j] = 0;
+            for (int j = 0; j < 128; ++j) acc[j] = 0.f;
             // Under the MMAs' operand traffic an access to shared memory takes 200 to 300 cycles, a look at a barrier as well: scales and the state of
             // the next block are asked for while a block is added, and used behind it.
             float sr = 0.f, sw0 = 0.f, sw1 = 0.f, f0 = 0.f, f1 = 0.f;
@@ -351,15 +360,15 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                 }
                 if (any) {
                     const uint32_t at = taddr + uint32_t(buf * kTileCols);
-                    const uint64_t g0 = pair_of(f0), g1 = kSwiGLU ? pair_of(f1) : g0;
-                    auto add_a = [&](int c, int pairs) {
+                    const float g0 = f0, g1 = kSwiGLU ? f1 : f0;
+                    auto add_a = [&](int c, int columns) {
 #pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            if (j < pairs) fma_pair(sum[c / 2 + j], a[2 * j], a[2 * j + 1], c < 64 ? g0 : g1);
+                        for (int j = 0; j < 32; ++j)
+                            if (j < columns) acc[c + j] = fmaf(__uint_as_float(a[j]), c < 64 ? g0 : g1, acc[c + j]);
                     };
                     auto add_b = [&](int c) {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) fma_pair(sum[c / 2 + j], b[2 * j], b[2 * j + 1], c < 64 ? g0 : g1);
+                        for (int j = 0; j < 16; ++j) acc[c + j] = fmaf(__uint_as_float(b[j]), c < 64 ? g0 : g1, acc[c + j]);
                     };
                     tmem_ld_wait();
                     tmem_ld32(at + 16, a);
@@ -367,14 +376,14 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                     add_b(0);
                     tmem_ld_wait();
                     tmem_ld16(at + 48, b);
-                    add_a(16, 16);
+                    add_a(16, 32);
                     tmem_ld_wait();
                     tmem_ld32(at + 64, a);
                     add_b(48);
                     tmem_ld_wait();
                     tmem_ld16(at + 96, b);
                     const bool next_done = block_done(&sh.done[stage], phase);
-                    add_a(64, 16);
+                    add_a(64, 32);
                     tmem_ld_wait();
                     tmem_ld16(at + 112, a);
                     add_b(96);
@@ -386,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                         tc_fence_after();
                         tmem_ld16(taddr + uint32_t((buf ^ 1) * kTileCols), b);
                     }
-                    add_a(112, 8);
+                    add_a(112, 16);
                 } else {
                     tc_fence_before();
                     if (lane == 0) arrive_read(empty_addr + uint32_t(buf) * 8u);
@@ -396,13 +405,8 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
             }
             if (!ok) break;
             if (!any) continue;
-            float acc[128];
-#pragma unroll
-            for (int j = 0; j < 64; ++j) {
-                acc[2 * j] = __uint_as_float(uint32_t(sum[j]));
-                acc[2 * j + 1] = __uint_as_float(uint32_t(sum[j] >> 32));
-            }
             constexpr int kCols = kSwiGLU ? 64 : 128;  // output columns of this thread
+            pieces_read();                             // the tile before, long past
             const int n0 = kSwiGLU ? t.nt * 128 + group * 64 : t.nt * kTileCols + group * 128;
             if (kSwiGLU) {
 #pragma unroll
@@ -435,31 +439,23 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                 const float per = __fdiv_rn(kLargest, m);  // sums do not lie on the border of two e4m3 values: a product will do
                 if (real && (kSwiGLU ? group == 0 : inside)) args.scales[row * args.n_blocks + wb] = __fdiv_rn(m, kLargest);
 #pragma unroll
-                for (int j = 0; j < kCols; j += 64) {
-                    pieces_read();
+                for (int j = 0; j < kCols; j += 16) {
+                    uint32_t q[4];
 #pragma unroll
-                    for (int i = 0; i < 64; i += 16) {
-                        uint32_t q[4];
-#pragma unroll
-                        for (int h = 0; h < 4; ++h) {
-                            const float* f = acc + j + i + 4 * h;
-                            q[h] = pack_e4m3(f[0] * per, f[1] * per, f[2] * per, f[3] * per);
-                        }
-                        *reinterpret_cast<uint4*>(piece + i) = make_uint4(q[0], q[1], q[2], q[3]);
+                    for (int h = 0; h < 4; ++h) {
+                        const float* f = acc + j + 4 * h;
+                        q[h] = pack_e4m3(f[0] * per, f[1] * per, f[2] * per, f[3] * per);
                     }
-                    if (real && n0 + j < args.n) send_piece(args.q + row * args.n + n0 + j, piece, min(64, args.n - n0 - j));
+                    *reinterpret_cast<uint4*>(piece + j) = make_uint4(q[0], q[1], q[2], q[3]);
                 }
+                if (real && n0 < args.n) send_piece(args.q + row * args.n + n0, piece, min(kCols, args.n - n0));
             } else {
 #pragma unroll
-                for (int j = 0; j < kCols; j += 32) {
-                    pieces_read();
-#pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        const float* f = acc + j + i;
-                        *reinterpret_cast<uint4*>(piece + i * 2) = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
-                    }
-                    if (real && n0 + j < args.n) send_piece(args.out + row * args.n + n0 + j, piece, 2 * min(32, args.n - n0 - j));
+                for (int j = 0; j < kCols; j += 8) {
+                    const float* f = acc + j;
+                    *reinterpret_cast<uint4*>(piece + j * 2) = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
                 }
+                if (real && n0 < args.n) send_piece(args.out + row * args.n + n0, piece, 2 * min(kCols, args.n - n0));
             }
         }
         asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // the rows have left shared memory and are written
