@@ -38,7 +38,7 @@ constexpr int kSlice = 32;                     // rows exchanged at a time, half
 template <int kTileRows>
 struct Shape {
     static constexpr int kStageBytes = kWeightBytes + kTileRows * 128;
-    static constexpr int kStages = kTileRows <= 32 ? 5 : kTileRows <= 64 ? 4 : 3;
+    static constexpr int kStages = kTileRows <= 32 ? 5 : 4;
     static constexpr int kBufs = kTmemCols / (2 * kTileRows) < 8 ? kTmemCols / (2 * kTileRows) : 8;
 };
 
@@ -60,7 +60,7 @@ template <int kTileRows>
 constexpr size_t smem_bytes() {
     return size_t(Shape<kTileRows>::kStages) * Shape<kTileRows>::kStageBytes + sizeof(Shared<kTileRows>);
 }
-static_assert(smem_bytes<32>() <= 232448 && smem_bytes<64>() <= 232448 && smem_bytes<128>() <= 232448, "shared memory of a CTA");
+static_assert(smem_bytes<32>() <= 232448 && smem_bytes<64>() <= 232448, "shared memory of a CTA");
 
 struct Tile {
     int expert, row0, rows, nt;
@@ -456,8 +456,7 @@ cudaError_t launch_tile(const Maps& maps, const Args& args, int ctas, int64_t un
 template <bool kSwiGLU, bool kQuantize>
 cudaError_t launch_mode(const Maps& maps, const Args& args, int tile, int ctas, int64_t units, int sms, cudaStream_t stream) {
     if (tile <= 32) return launch_tile<kSwiGLU, kQuantize, 32>(maps, args, ctas, units, sms, stream);
-    if (tile <= 64) return launch_tile<kSwiGLU, kQuantize, 64>(maps, args, ctas, units, sms, stream);
-    return launch_tile<kSwiGLU, kQuantize, 128>(maps, args, ctas, units, sms, stream);
+    return launch_tile<kSwiGLU, kQuantize, 64>(maps, args, ctas, units, sms, stream);
 }
 
 }  // namespace

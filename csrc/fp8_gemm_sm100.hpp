@@ -34,10 +34,10 @@ struct Args {
     uint32_t* status;               // 2 words: first error code, detail
     uint64_t timeout_ns;
 };
-// Many rows per expert: rows as M, pairs of CTAs (fp8_gemm_sm100.cu).  Weight boxes of 128 rows, 64 with SwiGLU.
+// Rows as M (fp8_gemm_sm100.cu).  Weight boxes of 128 rows, 64 with SwiGLU.
 cudaError_t launch(const Maps& maps, const Args& args, int grid, cudaStream_t stream);
 
-// Few rows per expert: weights as M, `tile` (32, 64 or 128) rows at most as N, the K axis split over clusters of `ctas` (1, 2, 4 or 8) CTAs
+// Few rows per expert: weights as M, `tile` (32 or 64) rows at most as N, the K axis split over clusters of `ctas` (1, 2, 4 or 8) CTAs
 // (fp8_gemm_few_sm100.cu).  `units`: tiles that the rows allow.  Weight boxes of 128 rows.
 cudaError_t launch_few(const Maps& maps, const Args& args, int tile, int ctas, int64_t units, int sms, cudaStream_t stream);
 int few_clusters(int ctas, int sms);

@@ -337,28 +337,34 @@ void check_i64(const OptTensor& t, const at::Tensor& a, int64_t entries, const c
                     " must be a contiguous int64 tensor of ", std::to_string(entries), " entries on the rows' device");
 }
 
-// Which kernel an 8-bit product runs: tile = 256: rows as M, pairs of CTAs; less: weights as M, so many rows at most as N, the K axis over
-// `ctas` CTAs.  `units`: tiles that the rows allow, whatever the offsets say.
+// Which kernel an 8-bit product runs.  tile = 128: rows as M (fp8_gemm_sm100.cu); 32 or 64: weights as M, so many rows at most as N, the K
+// axis over `ctas` CTAs (fp8_gemm_few_sm100.cu).  `units`: tiles that the rows allow, whatever the offsets say.
+//
+// The choice is the shortest of the times that these kernels have taken, whole passes over the tiles at a time.  us a block of 128 columns: rows
+// as M 0.62 on a few SMs and 0.69 on all; 32 rows as N 0.43 alone, 0.70 where all SMs stream weights from memory, 0.45 where L2 has
+// them; 64 rows 0.61 and 0.86.  Behind a tile's last block: 2.7, and 2.5 + 0.3 a CTA for the exchange.  32 experts of 7168 x 2048, up, us for 32
+// rows as N, 64, and rows as M: 32 rows an expert 157, 166, 172; 64 rows 199, 192, 174.  One matrix of 7168 x 4096: one row 14 over four
+// CTAs, 27 in one, 35; 128 rows 27, 21, 38.
 struct Fp8Choice {
     int64_t tile, ctas, units;
 };
 Fp8Choice choose_fp8(int64_t rows, int64_t experts, int64_t most, int64_t n_tiles, int64_t k_blocks, int64_t sms, int64_t tile, int64_t ctas) {
-    const int64_t holders = std::min(experts, rows), average = (rows + holders - 1) / holders;
-    if (experts == 1 || most <= 0 || most > rows) most = experts == 1 ? rows : rows - holders + 1;
+    const int64_t holders = std::min(experts, rows), average = std::max((rows + holders - 1) / holders, most > 0 && most <= 32 ? most : 1);
+    const auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
     Fp8Choice c{};
-    c.tile = tile > 0 ? tile : average > 192 ? 256 : most <= 32 || average <= 20 ? 32 : most <= 64 || average <= 40 ? 64 : 128;
-    c.units = (rows / std::min<int64_t>(c.tile, 128) + holders) * n_tiles;
-    const int64_t likely = holders * ((average + c.tile - 1) / c.tile) * n_tiles;
-    c.ctas = ctas > 0 ? ctas : 1;
-    if (ctas <= 0 && c.tile <= 128) {
-        // the split that is through first: whole passes of the clusters over the tiles, and about three blocks' time for the exchange
-        int64_t best = -1;
-        for (int64_t s = 1; s <= 8; s *= 2) {
-            const int64_t clusters = fp8::few_clusters(int(s), int(sms)), time = (likely + clusters - 1) / clusters * ((k_blocks + s - 1) / s + 3);
-            if (best < 0 || time < best) {
-                best = time;
-                c.ctas = s;
-            }
+    double best = -1;
+    for (const int64_t t : {int64_t(32), int64_t(64), int64_t(128)}) {
+        if (tile > 0 && t != tile) continue;
+        const int64_t tiles = up(average, t), units = holders * tiles * n_tiles;
+        for (int64_t s = 1; s <= (t == 128 ? 1 : 8); s *= 2) {
+            if (ctas > 0 && s != ctas && t != 128) continue;
+            const int64_t clusters = fp8::few_clusters(int(s), int(sms));
+            const double busy = double(std::min(units, clusters) * s) / double(sms);
+            const double block = t == 128 ? 0.62 + 0.07 * busy : t == 64 ? 0.61 + 0.25 * busy : tiles > 1 ? 0.45 : 0.43 + 0.27 * busy;
+            const double time = double(up(units, clusters)) * (double(up(k_blocks, s)) * block + (t == 128 ? 2.7 : 2.5 + 0.3 * double(s)));
+            if (best >= 0 && time >= best) continue;
+            best = time;
+            c = Fp8Choice{t, s, (rows / t + holders) * n_tiles};
         }
     }
     return c;
@@ -394,8 +400,8 @@ std::vector<at::Tensor> grouped_gemm_fp8(const at::Tensor& a, const at::Tensor& 
                         row_scale->dim() == 1 && row_scale->size(0) == rows,
                     "row_scale must be contiguous float32 [rows] on the rows' device (without swiglu)");
     TORCH_CHECK(max_expert_rows >= 0, "max_expert_rows must not be negative");
-    TORCH_CHECK((tile == 0 || tile == 32 || tile == 64 || tile == 128 || tile == 256) && (ctas == 0 || ctas == 1 || ctas == 2 || ctas == 4 || ctas == 8),
-                "tile must be 0, 32, 64, 128 or 256 and ctas 0, 1, 2, 4 or 8");
+    TORCH_CHECK((tile == 0 || tile == 32 || tile == 64 || tile == 128) && (ctas == 0 || ctas == 1 || ctas == 2 || ctas == 4 || ctas == 8),
+                "tile must be 0, 32, 64 or 128 and ctas 0, 1, 2, 4 or 8");
     check_status_tensor(status, a);
     c10::cuda::CUDAGuard guard(a.device());
     std::vector<at::Tensor> out;
@@ -430,10 +436,10 @@ std::vector<at::Tensor> grouped_gemm_fp8(const at::Tensor& a, const at::Tensor& 
     const int sms = sm_count();
     const Fp8Choice c = choose_fp8(rows, E, max_expert_rows, g.n_tiles, g.k_blocks, sms, tile, ctas);
     fp8::Maps maps{};
-    maps.weights = e4m3_map(w.data_ptr(), K, n, E * halves, swiglu && c.tile > 128 ? 64 : 128);
+    maps.weights = e4m3_map(w.data_ptr(), K, n, E * halves, swiglu && c.tile == 128 ? 64 : 128);
     for (int b = 0; b < 4; ++b) maps.rows[b] = e4m3_map(a.data_ptr(), K, rows, 0, 128 >> b);
     const auto stream = c10::cuda::getCurrentCUDAStream();
-    launched(c.tile > 128 ? fp8::launch(maps, g, int(std::min<int64_t>(sms, c.units)), stream) : fp8::launch_few(maps, g, int(c.tile), int(c.ctas), c.units, sms, stream),
+    launched(c.tile == 128 ? fp8::launch(maps, g, int(std::min<int64_t>(sms, c.units)), stream) : fp8::launch_few(maps, g, int(c.tile), int(c.ctas), c.units, sms, stream),
              "grouped_gemm_fp8");
     return out;
 }
@@ -449,6 +455,10 @@ void bind_ops(pybind11::module_& m) {
     m.def("sort_tokens", &sort_tokens, py::arg("x"), py::arg("slots"), py::arg("slot_map"), py::arg("scales"), py::arg("zero_padding"));
     m.def("unsort_tokens", &unsort_tokens, py::arg("y"), py::arg("slots"), py::arg("slot_map"), py::arg("weights"), py::arg("bias"));
     m.def("unsort_tokens_grad", &unsort_tokens_grad, py::arg("grad_out"), py::arg("y"), py::arg("slots"), py::arg("slot_map"), py::arg("weights"));
+    m.def("fp8_gemm_choice", [](int64_t rows, int64_t experts, int64_t most, int64_t n_tiles, int64_t k_blocks, int64_t sms) {
+        const Fp8Choice c = choose_fp8(rows, experts, most, n_tiles, k_blocks, sms, 0, 0);
+        return std::make_pair(c.tile, c.ctas);
+    });
     m.def("grouped_gemm_fp8", &grouped_gemm_fp8, py::arg("a"), py::arg("a_scales"), py::arg("w"), py::arg("w_scales"), py::arg("expert_offsets"),
           py::arg("expert_counts"), py::arg("row_scale"), py::arg("swiglu"), py::arg("quantize"), py::arg("max_expert_rows"), py::arg("status"), py::arg("tile") = 0, py::arg("ctas") = 0);
 }

@@ -136,7 +136,7 @@ def test_rows_that_do_not_exist(alignment, tail, quantize):
 
 
 @pytest.mark.parametrize("counts", [[1], [16], [17, 0, 40], [129, 300, 0, 5], [33, 64, 65, 128, 256, 257]])
-@pytest.mark.parametrize("tile,ctas", [(32, 1), (32, 2), (32, 4), (32, 8), (64, 1), (64, 2), (64, 8), (128, 1), (128, 4), (256, 1)])
+@pytest.mark.parametrize("tile,ctas", [(32, 1), (32, 2), (32, 4), (32, 8), (64, 1), (64, 2), (64, 8), (128, 1)])
 @pytest.mark.parametrize("K,n,swiglu,quantize,scaled", [(128, 48, False, False, True), (2064, 400, False, True, False), (1024, 384, True, True, False), (400, 144, True, False, False)])
 def test_every_kernel(counts, tile, ctas, K, n, swiglu, quantize, scaled):
     """Every tile and split of the K axis, also where a CTA's part of it is empty."""
