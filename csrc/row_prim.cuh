@@ -95,9 +95,22 @@ __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
     return lo | hi << 16;
 }
-// v in units of its block's scale: v * 448 / m with m = the block's largest.  Exact ties are common where v is a product of two
-// 16-bit values (v * 448 is exact then), and a correctly rounded quotient keeps them ties; a reciprocal does not.
-__device__ __forceinline__ float quotient(float v, float m) { return __fdiv_rn(v * kLargest, m); }
+// Values in units of their block's scale: v * 448 / m with m = the block's largest.  Exact ties are common where v is a product of two
+// 16-bit values (v * 7 is exact then), and they have to stay ties.  q0 = r * (1 / d), off by 2^-22 at most; its remainder r - q0 * d is exact
+// in a fused multiply-add; q0 plus the remainder over d is the quotient to within its rounding.  Where that is a tie, 5 significant bits,
+// it is hit; where not, it lies 2^-21 from one at least, since r and d have 19 and 16 bits.  (__fdiv_rn: 51 us instead of 44 for 4096 rows of 7168.)
+struct Quotient {
+    float d, inverse;
+    __device__ __forceinline__ explicit Quotient(float m) {
+        d = m * 0x1p-10f;  // 448 = 7 / 16 * 2^10: neither side overflows
+        inverse = __frcp_rn(d);
+        if (inverse == 0.f) d = 0.f;  // an infinite block: finite values are 0 of it, infinities NaN
+    }
+    __device__ __forceinline__ float operator()(float v) const {
+        const float r = v * 0.4375f, q0 = r * inverse;
+        return fmaf(fmaf(-q0, d, r), inverse, q0);
+    }
+};
 
 template <int kWidth>
 __device__ __forceinline__ float group_max(float v) {

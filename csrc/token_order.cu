@@ -42,29 +42,45 @@ __device__ __forceinline__ void cluster_barrier() {
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 
+// Up to kKept * 32 choices a warp stay in registers between the two walks; longer runs are read again.
+constexpr int kKept = 8;
+
+template <bool kInRegisters>
 __global__ void __launch_bounds__(kPlanThreads, 1) plan_kernel(const PlanArgs a, int ctas, int64_t per_warp) {
     extern __shared__ __align__(16) uint8_t smem[];
     PlanShared& sh = *reinterpret_cast<PlanShared*>(smem);
     int* hist = reinterpret_cast<int*>(smem + sizeof(PlanShared));  // [warps][experts]
     const int E = a.experts, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t cta = ctas > 1 ? cluster_rank() : 0;
-    for (int i = tid; i < kPlanWarps * E; i += kPlanThreads) hist[i] = 0;
-    __syncthreads();
-
     const int64_t first = (int64_t(cta) * kPlanWarps + warp) * per_warp;
     const int64_t last = min(a.choices, first + per_warp);
     int* mine = hist + warp * E;
-    for (int64_t at = first; at < last; at += 32) {
-        const int64_t i = at + lane;
+    auto read = [&](int64_t i) -> int {
         int64_t id = i < last ? a.topk_idx[i] : -1;
         if (id < -1 || id >= E) {
             if (atomicCAS(a.status, 0u, uint32_t(kBadExpertId)) == 0u) a.status[1] = uint32_t(i);
             id = -1;
         }
-        const int e = int(id);
+        return int(id);
+    };
+    int kept[kInRegisters ? kKept : 1];
+    if (kInRegisters) {
+#pragma unroll
+        for (int j = 0; j < kKept; ++j) kept[j] = read(first + j * 32 + lane);
+    }
+    for (int i = tid; i < kPlanWarps * E; i += kPlanThreads) hist[i] = 0;
+    __syncthreads();
+    auto count_32 = [&](int e) {
         const uint32_t same = __match_any_sync(0xffffffffu, e);
         if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
         __syncwarp();
+    };
+    if (kInRegisters) {
+#pragma unroll
+        for (int j = 0; j < kKept; ++j)
+            if (first + j * 32 < last) count_32(kept[j]);
+    } else {
+        for (int64_t at = first; at < last; at += 32) count_32(read(at + lane));
     }
     __syncthreads();
     for (int e = tid; e < E; e += kPlanThreads) {
@@ -123,21 +139,25 @@ __global__ void __launch_bounds__(kPlanThreads, 1) plan_kernel(const PlanArgs a,
     const int64_t end = sh.scan[kPlanWarps];
     for (int64_t s = end + int64_t(cta) * kPlanThreads + tid; s < a.capacity; s += int64_t(ctas) * kPlanThreads) a.slot_map[s] = -1;
 
-    for (int64_t at = first; at < last; at += 32) {
+    auto place_32 = [&](int64_t at, int e) {
         const int64_t i = at + lane;
-        const int64_t id = i < last ? a.topk_idx[i] : -1;
-        const int e = id < 0 || id >= E ? -1 : int(id);
         const uint32_t same = __match_any_sync(0xffffffffu, e);
-        const int leader = __ffs(same) - 1;
         int slot = -1;
         if (e >= 0) slot = sh.base[e] + mine[e] + __popc(same & ((1u << lane) - 1));
         __syncwarp();
-        if (e >= 0 && lane == leader) mine[e] += __popc(same);
+        if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
         __syncwarp();
         if (i < last) {
             a.slots[i] = slot;
             if (slot >= 0) a.slot_map[slot] = int(i);
         }
+    };
+    if (kInRegisters) {
+#pragma unroll
+        for (int j = 0; j < kKept; ++j)
+            if (first + j * 32 < last) place_32(first + j * 32, kept[j]);
+    } else {
+        for (int64_t at = first; at < last; at += 32) place_32(at, read(at + lane));
     }
     if (ctas > 1) cluster_barrier();  // nobody's totals go away while another CTA reads them
 }
@@ -220,6 +240,21 @@ __device__ __forceinline__ void store8(T* row, int c, int hidden, const float* f
     }
 }
 
+// Eight columns as they lie in memory; `get` converts them.  Loads of several rows stay in flight only if none is converted in between.
+template <typename T, bool kAligned>
+struct Eight {
+    Raw8<T> raw;
+    __device__ __forceinline__ void load(const T* row, int c, int hidden) {
+        if (kAligned) {
+            raw.load(row + c);
+        } else {
+            float f[8];
+            load8<T, false>(row, c, hidden, f);
+            raw.set(f);
+        }
+    }
+};
+
 template <typename T, bool kAligned>
 __global__ void __launch_bounds__(256) unsort_kernel(const UnsortArgs a, int pieces) {
     const int lane = threadIdx.x & 31;
@@ -233,20 +268,25 @@ __global__ void __launch_bounds__(256) unsort_kernel(const UnsortArgs a, int pie
     const T* y = static_cast<const T*>(a.y);
     float acc[8] = {};
     for (int k0 = 0; k0 < a.topk; k0 += 8) {
-        float f[8][8];
-        bool real[8];
+        Eight<T, kAligned> f[8];
+        uint32_t real = 0;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             const int slot = k0 + k < a.topk ? __shfl_sync(0xffffffffu, my_slot, (k0 + k) & 31) : -1;
-            real[k] = uint32_t(slot) < uint64_t(a.capacity) && inside;
-            if (real[k]) load8<T, kAligned>(y + int64_t(slot) * a.hidden, c, a.hidden, f[k]);
+            f[k].raw.clear();
+            if (uint32_t(slot) < uint64_t(a.capacity) && inside) {
+                f[k].load(y + int64_t(slot) * a.hidden, c, a.hidden);
+                real |= 1u << k;
+            }
         }
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             const float w = __shfl_sync(0xffffffffu, my_weight, (k0 + k) & 31);
-            if (!real[k]) continue;
+            float v[8];
+            f[k].raw.get(v);
+            if ((real >> k & 1u) == 0) continue;  // a masked choice's weight may be anything
 #pragma unroll
-            for (int j = 0; j < 8; ++j) acc[j] += w * f[k][j];
+            for (int j = 0; j < 8; ++j) acc[j] += w * v[j];
         }
     }
     if (!inside) return;
@@ -345,7 +385,8 @@ cudaError_t launch_plan(const PlanArgs& a, cudaStream_t stream) {
     const int64_t warps = int64_t(ctas) * kPlanWarps;
     const int64_t per_warp = ((a.choices + warps - 1) / warps + 31) / 32 * 32;
     const size_t smem = sizeof(PlanShared) + size_t(kPlanWarps) * a.experts * sizeof(int);
-    cudaError_t e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(PlanShared) + size_t(kPlanWarps) * kMaxExperts * sizeof(int)));
+    auto* fn = per_warp <= 32 * kKept ? plan_kernel<true> : plan_kernel<false>;
+    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(PlanShared) + size_t(kPlanWarps) * kMaxExperts * sizeof(int)));
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(unsigned(ctas));
@@ -359,7 +400,7 @@ cudaError_t launch_plan(const PlanArgs& a, cudaStream_t stream) {
     attr[0].val.clusterDim.z = 1;
     config.attrs = attr;
     config.numAttrs = 1;
-    return cudaLaunchKernelEx(&config, plan_kernel, a, ctas, per_warp);
+    return cudaLaunchKernelEx(&config, fn, a, ctas, per_warp);
 }
 
 cudaError_t launch_sort(const SortArgs& a, cudaStream_t stream) {

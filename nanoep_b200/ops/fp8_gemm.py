@@ -8,7 +8,8 @@ from __future__ import annotations
 
 import torch
 
-from .grouped_gemm import _ext, operator_status
+from ..utils.build import load_extension as _ext
+from .grouped_gemm import operator_status
 
 BLOCK = 128
 LARGEST = 448.0  # of e4m3

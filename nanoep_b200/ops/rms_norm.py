@@ -10,7 +10,8 @@ from typing import NamedTuple
 
 import torch
 
-from .grouped_gemm import _ext, refuse_captured_gradients
+from ..utils.build import load_extension as _ext
+from .grouped_gemm import refuse_captured_gradients
 
 
 class NormResult(NamedTuple):

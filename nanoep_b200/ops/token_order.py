@@ -11,7 +11,8 @@ from typing import NamedTuple
 
 import torch
 
-from .grouped_gemm import _ext, operator_status, refuse_captured_gradients
+from ..utils.build import load_extension as _ext
+from .grouped_gemm import operator_status, refuse_captured_gradients
 
 
 class TokenOrder(NamedTuple):
