@@ -18,6 +18,7 @@
 #include <algorithm>
 
 #include "fp8_prim.cuh"
+#include "launch_once.hpp"
 #include "row_prim.cuh"
 #include "tc_prim.cuh"
 
@@ -436,7 +437,8 @@ template <bool kSwiGLU, bool kQuantize, int kTileRows>
 cudaError_t launch_tile(const Maps& maps, const Args& args, int ctas, int64_t units, int sms, cudaStream_t stream) {
     auto* fn = fp8_gemm_few_kernel<kSwiGLU, kQuantize, kTileRows>;
     constexpr size_t kBytes = smem_bytes<kTileRows>();
-    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kBytes));
+    static std::atomic<uint64_t> raised{0};
+    const cudaError_t e = raise_shared_limit(fn, int(kBytes), raised);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t config{};
     config.blockDim = dim3(kThreads);

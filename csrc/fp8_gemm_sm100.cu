@@ -19,6 +19,7 @@
 #include "fp8_gemm_sm100.hpp"
 
 #include "fp8_prim.cuh"
+#include "launch_once.hpp"
 #include "row_prim.cuh"
 #include "tc_prim.cuh"
 
@@ -471,7 +472,8 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
 template <bool kSwiGLU, bool kQuantize>
 cudaError_t launch_mode(const Maps& maps, const Args& args, int grid, cudaStream_t stream) {
     auto* fn = fp8_gemm_kernel<kSwiGLU, kQuantize>;
-    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes));
+    static std::atomic<uint64_t> raised{0};
+    const cudaError_t e = raise_shared_limit(fn, int(kSmemBytes), raised);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(unsigned(grid));

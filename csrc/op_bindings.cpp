@@ -3,6 +3,7 @@
 #include "op_api.hpp"
 
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -18,6 +19,11 @@ namespace {
 static_assert(order::kMaxTopk == 32 && order::kMaxExperts == 1024 && fp8::kMaxExperts == 1024, "limits named in messages");
 
 using OptTensor = c10::optional<at::Tensor>;
+
+// A tensor on the device of `like` without the dispatcher: a small call's time is the host's, about a microsecond a tensor.
+at::Tensor make_empty(at::IntArrayRef sizes, at::ScalarType dtype, const at::Tensor& like) {
+    return at::Tensor(at::detail::empty_cuda(sizes, dtype, like.device(), c10::nullopt));
+}
 
 // Element types in the numbering that norm::Type and order::Type share.
 int row_type(const at::Tensor& t, const char* name) {
@@ -74,13 +80,13 @@ std::vector<OptTensor> rms_norm(const at::Tensor& x, const at::Tensor& weight, c
     TORCH_CHECK(quantize || keep, "neither the rows nor their 8-bit form is asked for");
     c10::cuda::CUDAGuard guard(x.device());
     OptTensor y, q, scales, stream, rstd;
-    if (keep) y = at::empty_like(x);
+    if (keep) y = make_empty(x.sizes(), x.scalar_type(), x);
     if (quantize) {
-        q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
-        scales = at::empty({x.size(0), blocks_of(x.size(1))}, x.options().dtype(at::kFloat));
+        q = make_empty(x.sizes(), at::kFloat8_e4m3fn, x);
+        scales = make_empty({x.size(0), blocks_of(x.size(1))}, at::kFloat, x);
     }
-    if (residual.has_value()) stream = at::empty_like(x);
-    if (save) rstd = at::empty({x.size(0)}, x.options().dtype(at::kFloat));
+    if (residual.has_value()) stream = make_empty(x.sizes(), x.scalar_type(), x);
+    if (save) rstd = make_empty({x.size(0)}, at::kFloat, x);
     if (x.size(0) > 0) {
         norm::NormArgs a{};
         a.x = x.data_ptr();
@@ -112,11 +118,11 @@ std::pair<at::Tensor, at::Tensor> rms_norm_grad(const at::Tensor& grad_y, const 
     TORCH_CHECK(rstd.is_cuda() && rstd.device() == h.device() && rstd.scalar_type() == at::kFloat && rstd.is_contiguous() && rstd.dim() == 1 && rstd.size(0) == h.size(0),
                 "rstd must be float32 [tokens] on the rows' device");
     c10::cuda::CUDAGuard guard(h.device());
-    at::Tensor grad_x = at::empty_like(h);
+    at::Tensor grad_x = make_empty(h.sizes(), h.scalar_type(), h);
     if (h.size(0) == 0) return {grad_x, at::zeros_like(weight)};
-    at::Tensor grad_weight = at::empty_like(weight);
+    at::Tensor grad_weight = make_empty(weight.sizes(), weight.scalar_type(), h);
     const int sms = sm_count();
-    at::Tensor partial = at::empty({norm::grad_blocks(h.size(0), sms), h.size(1)}, h.options().dtype(at::kFloat));
+    at::Tensor partial = make_empty({norm::grad_blocks(h.size(0), sms), h.size(1)}, at::kFloat, h);
     norm::NormGradArgs a{};
     a.grad_y = grad_y.data_ptr();
     a.h = h.data_ptr();
@@ -139,8 +145,8 @@ std::pair<at::Tensor, at::Tensor> quantize_rows(const at::Tensor& x) {
     check_hidden(x);
     const int type = row_type(x, "x");
     c10::cuda::CUDAGuard guard(x.device());
-    at::Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
-    at::Tensor scales = at::empty({x.size(0), blocks_of(x.size(1))}, x.options().dtype(at::kFloat));
+    at::Tensor q = make_empty(x.sizes(), at::kFloat8_e4m3fn, x);
+    at::Tensor scales = make_empty({x.size(0), blocks_of(x.size(1))}, at::kFloat, x);
     if (x.size(0) > 0) {
         norm::QuantizeArgs a{};
         a.x = x.data_ptr();
@@ -170,9 +176,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> plan_tokens(const at:
     const int64_t capacity = (choices + (std::min(experts, choices) + 1) * (alignment - 1)) / alignment * alignment;
     TORCH_CHECK(capacity < (int64_t(1) << 31), "at most 2^31 - 1 rows");
     c10::cuda::CUDAGuard guard(topk_idx.device());
-    const at::TensorOptions i32 = topk_idx.options().dtype(at::kInt);
-    at::Tensor slots = at::empty(topk_idx.sizes(), i32), slot_map = at::empty({capacity}, i32);
-    at::Tensor counts = at::empty({experts}, topk_idx.options()), offsets = at::empty({experts + 1}, topk_idx.options());
+    at::Tensor slots = make_empty(topk_idx.sizes(), at::kInt, topk_idx), slot_map = make_empty({capacity}, at::kInt, topk_idx);
+    at::Tensor counts = make_empty({experts}, at::kLong, topk_idx), offsets = make_empty({experts + 1}, at::kLong, topk_idx);
     order::PlanArgs a{};
     a.topk_idx = topk_idx.data_ptr<int64_t>();
     a.slots = slots.data_ptr<int>();
@@ -210,9 +215,9 @@ std::pair<at::Tensor, OptTensor> sort_tokens(const at::Tensor& x, const at::Tens
                     "scales must be contiguous float32 [tokens, blocks] on the rows' device");
     c10::cuda::CUDAGuard guard(x.device());
     const int64_t capacity = slot_map.size(0);
-    at::Tensor rows = at::empty({capacity, x.size(1)}, x.options());
+    at::Tensor rows = make_empty({capacity, x.size(1)}, x.scalar_type(), x);
     OptTensor row_scales;
-    if (scales.has_value()) row_scales = at::empty({capacity, scales->size(1)}, scales->options());
+    if (scales.has_value()) row_scales = make_empty({capacity, scales->size(1)}, at::kFloat, x);
     order::SortArgs a{};
     a.x = x.data_ptr();
     a.rows = rows.data_ptr();
@@ -251,7 +256,7 @@ at::Tensor unsort_tokens(const at::Tensor& y, const at::Tensor& slots, const at:
                         bias->size(0) == slots.size(0) && bias->size(1) == y.size(1),
                     "bias must be a contiguous [tokens, hidden] tensor of y's type and device");
     c10::cuda::CUDAGuard guard(y.device());
-    at::Tensor out = at::empty({slots.size(0), y.size(1)}, y.options());
+    at::Tensor out = make_empty({slots.size(0), y.size(1)}, y.scalar_type(), y);
     if (slots.size(0) == 0) return out;
     order::UnsortArgs a{};
     a.y = y.data_ptr();
@@ -280,9 +285,9 @@ std::pair<at::Tensor, OptTensor> unsort_tokens_grad(const at::Tensor& grad_out, 
     TORCH_CHECK(grad_out.device() == y.device() && grad_out.scalar_type() == y.scalar_type() && grad_out.size(0) == slots.size(0) && grad_out.size(1) == y.size(1),
                 "grad_out must be a contiguous [tokens, hidden] tensor of y's type and device");
     c10::cuda::CUDAGuard guard(y.device());
-    at::Tensor grad_y = at::empty_like(y);
+    at::Tensor grad_y = make_empty(y.sizes(), y.scalar_type(), y);
     OptTensor grad_weights;
-    if (weights.has_value()) grad_weights = at::empty_like(*weights);
+    if (weights.has_value()) grad_weights = make_empty(weights->sizes(), at::kFloat, y);
     order::UnsortGradArgs a{};
     a.grad_out = grad_out.data_ptr();
     a.y = y.data_ptr();
@@ -406,10 +411,10 @@ std::vector<at::Tensor> grouped_gemm_fp8(const at::Tensor& a, const at::Tensor& 
     c10::cuda::CUDAGuard guard(a.device());
     std::vector<at::Tensor> out;
     if (quantize) {
-        out.push_back(at::empty({rows, n}, a.options()));
-        out.push_back(at::empty({rows, nb}, a_scales.options()));
+        out.push_back(make_empty({rows, n}, at::kFloat8_e4m3fn, a));
+        out.push_back(make_empty({rows, nb}, at::kFloat, a));
     } else {
-        out.push_back(at::empty({rows, n}, a.options().dtype(at::kBFloat16)));
+        out.push_back(make_empty({rows, n}, at::kBFloat16, a));
     }
     if (rows == 0) return out;
     fp8::Args g{};

@@ -5,6 +5,7 @@
 // run.  offset(e) = sum of the counts in front, each rounded up to `alignment`.
 #include "token_order.hpp"
 
+#include "launch_once.hpp"
 #include "row_prim.cuh"
 
 namespace nep {
@@ -16,7 +17,8 @@ using namespace rows;
 // ------------------------------------------------------------------------------------------------ plan
 // One cluster.  Every warp owns a run of neighbouring choices and counts it by expert; prefixes over warps and CTAs turn the
 // counts into each warp's first slots; the warps then walk their runs again and hand the slots out.  Equal experts within 32
-// choices are found by a match over the warp, so there are no atomics and the order is that of the choices.
+// choices are found by a vote per bit of their id, so there are no atomics and the order is that of the choices.  (With the warp's match
+// instruction, which takes turns with every other access to shared memory, 32768 choices took 16.7 us instead of 12.8.)
 constexpr int kPlanThreads = 1024, kPlanWarps = kPlanThreads / 32, kMaxPlanCtas = 8;
 
 struct PlanShared {
@@ -42,6 +44,17 @@ __device__ __forceinline__ void cluster_barrier() {
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 
+// Lanes that hold the same expert as this one; `bits` for ids up to the number of experts (masked choices hold that).
+__device__ __forceinline__ uint32_t same_expert(int e, int bits) {
+    uint32_t same = 0xffffffffu;
+    for (int b = 0; b < bits; ++b) {
+        const bool set = (e >> b & 1) != 0;
+        const uint32_t votes = __ballot_sync(0xffffffffu, set);
+        same &= set ? votes : ~votes;
+    }
+    return same;
+}
+
 // Up to kKept * 32 choices a warp stay in registers between the two walks; longer runs are read again.
 constexpr int kKept = 8;
 
@@ -55,40 +68,46 @@ __global__ void __launch_bounds__(kPlanThreads, 1) plan_kernel(const PlanArgs a,
     const int64_t first = (int64_t(cta) * kPlanWarps + warp) * per_warp;
     const int64_t last = min(a.choices, first + per_warp);
     int* mine = hist + warp * E;
+    const int bits = 32 - __clz(E);
     auto read = [&](int64_t i) -> int {
-        int64_t id = i < last ? a.topk_idx[i] : -1;
-        if (id < -1 || id >= E) {
-            if (atomicCAS(a.status, 0u, uint32_t(kBadExpertId)) == 0u) a.status[1] = uint32_t(i);
-            id = -1;
-        }
-        return int(id);
+        const int64_t id = i < last ? a.topk_idx[i] : -1;
+        if (id >= 0 && id < E) return int(id);
+        if (id != -1 && atomicCAS(a.status, 0u, uint32_t(kBadExpertId)) == 0u) a.status[1] = uint32_t(i);
+        return E;
     };
     int kept[kInRegisters ? kKept : 1];
+    uint32_t kept_same[kInRegisters ? kKept : 1];
     if (kInRegisters) {
 #pragma unroll
         for (int j = 0; j < kKept; ++j) kept[j] = read(first + j * 32 + lane);
     }
     for (int i = tid; i < kPlanWarps * E; i += kPlanThreads) hist[i] = 0;
     __syncthreads();
-    auto count_32 = [&](int e) {
-        const uint32_t same = __match_any_sync(0xffffffffu, e);
-        if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
+    auto count_32 = [&](int e) -> uint32_t {
+        const uint32_t same = same_expert(e, bits);
+        if (e < E && lane == __ffs(same) - 1) mine[e] += __popc(same);
         __syncwarp();
+        return same;
     };
     if (kInRegisters) {
 #pragma unroll
         for (int j = 0; j < kKept; ++j)
-            if (first + j * 32 < last) count_32(kept[j]);
+            if (first + j * 32 < last) kept_same[j] = count_32(kept[j]);
     } else {
         for (int64_t at = first; at < last; at += 32) count_32(read(at + lane));
     }
     __syncthreads();
     for (int e = tid; e < E; e += kPlanThreads) {
         int run = 0;
-        for (int w = 0; w < kPlanWarps; ++w) {
-            const int n = hist[w * E + e];
-            hist[w * E + e] = run;
-            run += n;
+        for (int w0 = 0; w0 < kPlanWarps; w0 += 8) {
+            int n[8];
+#pragma unroll
+            for (int w = 0; w < 8; ++w) n[w] = hist[(w0 + w) * E + e];
+#pragma unroll
+            for (int w = 0; w < 8; ++w) {
+                hist[(w0 + w) * E + e] = run;
+                run += n[w];
+            }
         }
         sh.total[e] = run;
     }
@@ -139,13 +158,12 @@ __global__ void __launch_bounds__(kPlanThreads, 1) plan_kernel(const PlanArgs a,
     const int64_t end = sh.scan[kPlanWarps];
     for (int64_t s = end + int64_t(cta) * kPlanThreads + tid; s < a.capacity; s += int64_t(ctas) * kPlanThreads) a.slot_map[s] = -1;
 
-    auto place_32 = [&](int64_t at, int e) {
+    auto place_32 = [&](int64_t at, int e, uint32_t same) {
         const int64_t i = at + lane;
-        const uint32_t same = __match_any_sync(0xffffffffu, e);
         int slot = -1;
-        if (e >= 0) slot = sh.base[e] + mine[e] + __popc(same & ((1u << lane) - 1));
+        if (e < E) slot = sh.base[e] + mine[e] + __popc(same & ((1u << lane) - 1));
         __syncwarp();
-        if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
+        if (e < E && lane == __ffs(same) - 1) mine[e] += __popc(same);
         __syncwarp();
         if (i < last) {
             a.slots[i] = slot;
@@ -155,9 +173,12 @@ __global__ void __launch_bounds__(kPlanThreads, 1) plan_kernel(const PlanArgs a,
     if (kInRegisters) {
 #pragma unroll
         for (int j = 0; j < kKept; ++j)
-            if (first + j * 32 < last) place_32(first + j * 32, kept[j]);
+            if (first + j * 32 < last) place_32(first + j * 32, kept[j], kept_same[j]);
     } else {
-        for (int64_t at = first; at < last; at += 32) place_32(at, read(at + lane));
+        for (int64_t at = first; at < last; at += 32) {
+            const int e = read(at + lane);
+            place_32(at, e, same_expert(e, bits));
+        }
     }
     if (ctas > 1) cluster_barrier();  // nobody's totals go away while another CTA reads them
 }
@@ -273,18 +294,17 @@ __global__ void __launch_bounds__(256) unsort_kernel(const UnsortArgs a, int pie
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             const int slot = k0 + k < a.topk ? __shfl_sync(0xffffffffu, my_slot, (k0 + k) & 31) : -1;
+            const bool there = uint32_t(slot) < uint64_t(a.capacity);
+            real |= uint32_t(there) << k;
             f[k].raw.clear();
-            if (uint32_t(slot) < uint64_t(a.capacity) && inside) {
-                f[k].load(y + int64_t(slot) * a.hidden, c, a.hidden);
-                real |= 1u << k;
-            }
+            if (there && inside) f[k].load(y + int64_t(slot) * a.hidden, c, a.hidden);
         }
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             const float w = __shfl_sync(0xffffffffu, my_weight, (k0 + k) & 31);
+            if ((real >> k & 1u) == 0) continue;  // a masked choice's weight may be anything
             float v[8];
             f[k].raw.get(v);
-            if ((real >> k & 1u) == 0) continue;  // a masked choice's weight may be anything
 #pragma unroll
             for (int j = 0; j < 8; ++j) acc[j] += w * v[j];
         }
@@ -386,7 +406,8 @@ cudaError_t launch_plan(const PlanArgs& a, cudaStream_t stream) {
     const int64_t per_warp = ((a.choices + warps - 1) / warps + 31) / 32 * 32;
     const size_t smem = sizeof(PlanShared) + size_t(kPlanWarps) * a.experts * sizeof(int);
     auto* fn = per_warp <= 32 * kKept ? plan_kernel<true> : plan_kernel<false>;
-    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(PlanShared) + size_t(kPlanWarps) * kMaxExperts * sizeof(int)));
+    static std::atomic<uint64_t> raised[2];
+    const cudaError_t e = raise_shared_limit(fn, int(sizeof(PlanShared) + size_t(kPlanWarps) * kMaxExperts * sizeof(int)), raised[per_warp <= 32 * kKept]);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(unsigned(ctas));
