@@ -440,6 +440,7 @@ std::vector<at::Tensor> grouped_gemm_fp8(const at::Tensor& a, const at::Tensor& 
     g.timeout_ns = uint64_t(5e9);
     const int sms = sm_count();
     const Fp8Choice c = choose_fp8(rows, E, max_expert_rows, g.n_tiles, g.k_blocks, sms, tile, ctas);
+    TORCH_CHECK(c.units < (int64_t(1) << 31), "too many output tiles for one call");
     fp8::Maps maps{};
     maps.weights = e4m3_map(w.data_ptr(), K, n, E * halves, swiglu && c.tile == 128 ? 64 : 128);
     for (int b = 0; b < 4; ++b) maps.rows[b] = e4m3_map(a.data_ptr(), K, rows, 0, 128 >> b);
@@ -449,11 +450,108 @@ std::vector<at::Tensor> grouped_gemm_fp8(const at::Tensor& a, const at::Tensor& 
     return out;
 }
 
+// ------------------------------------------------------------------------------------------------ gradients
+// The operators as nodes of autograd's graph, in C++: a node of Python's costs the host 10 us a pass each way.
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// What the backward functions compute has no graph of its own, and accumulation nodes remember the stream of the graph that made them: one that
+// outlives into a capture ends the process.
+void check_backward(const char* name, const char* explicit_name) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), name, " is differentiable once: call without create_graph");
+    TORCH_CHECK(c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None, name, " is not differentiated inside a CUDA graph capture: call ",
+                explicit_name, " there");
+}
+
+at::Tensor dense(const at::Tensor& t) { return t.defined() ? t.contiguous() : t; }
+OptTensor optional(const at::Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+
+struct NormNode : torch::autograd::Function<NormNode> {
+    // y, then the stream where there is a residual, then q and scales, then rstd
+    static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight, const OptTensor& residual, double eps, bool quantize) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const auto out = rms_norm(x, weight, residual, eps, quantize, true, true);
+        ctx->saved_data["stream"] = residual.has_value();
+        ctx->save_for_backward({residual.has_value() ? *out[3] : x, weight, *out[4]});
+        ctx->set_materialize_grads(false);
+        variable_list all{*out[0]}, fixed;
+        if (residual.has_value()) all.push_back(*out[3]);
+        if (quantize) fixed = {*out[1], *out[2]};
+        fixed.push_back(*out[4]);
+        all.insert(all.end(), fixed.begin(), fixed.end());
+        ctx->mark_non_differentiable(fixed);
+        return all;
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        check_backward("rms_norm", "rms_norm_grad");
+        const bool stream = ctx->saved_data["stream"].toBool();
+        const at::Tensor grad_y = dense(grads[0]), grad_stream = stream ? dense(grads[1]) : at::Tensor();
+        at::Tensor grad_x = grad_stream, grad_weight;
+        if (grad_y.defined()) {
+            const auto saved = ctx->get_saved_variables();
+            std::tie(grad_x, grad_weight) = rms_norm_grad(grad_y, saved[0], saved[1], saved[2], optional(grad_stream));
+        }
+        return {grad_x, grad_weight, stream ? grad_x : at::Tensor(), at::Tensor(), at::Tensor()};
+    }
+};
+
+struct SortNode : torch::autograd::Function<SortNode> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& slots, const at::Tensor& slot_map, bool zero_padding) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        ctx->save_for_backward({slots, slot_map});
+        return sort_tokens(x, slots, slot_map, {}, zero_padding).first;
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        check_backward("sort_tokens", "sort_tokens_grad");
+        const auto saved = ctx->get_saved_variables();
+        return {unsort_tokens(dense(grads[0]), saved[0], saved[1], {}, {}), at::Tensor(), at::Tensor(), at::Tensor()};
+    }
+};
+
+struct UnsortNode : torch::autograd::Function<UnsortNode> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& y, const at::Tensor& slots, const at::Tensor& slot_map, const OptTensor& weights, const OptTensor& bias) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        ctx->saved_data["weighted"] = weights.has_value();
+        ctx->saved_data["biased"] = bias.has_value();
+        ctx->save_for_backward({y, slots, slot_map, weights.has_value() ? *weights : at::Tensor()});
+        return unsort_tokens(y, slots, slot_map, weights, bias);
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        check_backward("unsort_tokens", "unsort_tokens_grad");
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor grad_out = dense(grads[0]);
+        at::Tensor grad_y, grad_weights;
+        if (ctx->needs_input_grad(0) || (ctx->saved_data["weighted"].toBool() && ctx->needs_input_grad(3))) {
+            const auto both = unsort_tokens_grad(grad_out, saved[0], saved[1], saved[2], optional(saved[3]));
+            grad_y = both.first;
+            if (both.second.has_value()) grad_weights = *both.second;
+        }
+        return {grad_y, at::Tensor(), at::Tensor(), grad_weights, ctx->saved_data["biased"].toBool() ? grad_out : at::Tensor()};
+    }
+};
+
 }  // namespace
 
 void bind_ops(pybind11::module_& m) {
     namespace py = pybind11;
     m.def("rms_norm", &rms_norm, py::arg("x"), py::arg("weight"), py::arg("residual"), py::arg("eps"), py::arg("quantize"), py::arg("keep"), py::arg("save"));
+    m.def("rms_norm_node", [](const at::Tensor& x, const at::Tensor& weight, const OptTensor& residual, double eps, bool quantize) -> std::vector<OptTensor> {
+        const auto out = NormNode::apply(x, weight, residual, eps, quantize);
+        size_t at = 1;
+        std::vector<OptTensor> named(5);
+        named[0] = out[0];
+        if (residual.has_value()) named[3] = out[at++];
+        if (quantize) named[1] = out[at], named[2] = out[at + 1];
+        named[4] = out.back();
+        return named;
+    });
+    m.def("sort_tokens_node", [](const at::Tensor& x, const at::Tensor& slots, const at::Tensor& slot_map, bool zero_padding) {
+        return SortNode::apply(x, slots, slot_map, zero_padding);
+    });
+    m.def("unsort_tokens_node", [](const at::Tensor& y, const at::Tensor& slots, const at::Tensor& slot_map, const OptTensor& weights, const OptTensor& bias) {
+        return UnsortNode::apply(y, slots, slot_map, weights, bias);
+    });
     m.def("rms_norm_grad", &rms_norm_grad, py::arg("grad_y"), py::arg("h"), py::arg("weight"), py::arg("rstd"), py::arg("grad_stream"));
     m.def("quantize_rows", &quantize_rows, py::arg("x"));
     m.def("plan_tokens", &plan_tokens, py::arg("topk_idx"), py::arg("num_experts"), py::arg("alignment"), py::arg("status"));

@@ -58,7 +58,8 @@ def grouped_gemm_fp8(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w
     expert_offsets: int64 ``[E + 1]``, not falling, from 0 to at most ``rows``, of any alignment; rows behind the last are not written.
     ``expert_counts`` (int64 ``[E]``): only so many rows of each range exist, the others are neither read nor written.
     ``row_scale`` (fp32 ``[rows]``, not with ``swiglu``) multiplies each output row before it is rounded.
-    ``max_expert_rows`` (0 = unknown): no expert holds more rows; the choice of the tile goes by it, the result does not.
+    ``max_expert_rows`` (0 = unknown): no expert holds more rows; the choice of the tile goes by it, the result only in
+    its rounding.
     """
     if w.dim() == 2:
         w, w_scales = w[None], w_scales[None]

@@ -33,13 +33,13 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tensor | 
     is normalised, so that the norm of the returned ``residual`` is the same.  ``quantize``: also in e4m3, ``q * scales = y`` with
     ``scales = max |y| / 448`` of each 128 columns (at least 1e-30 / 448 in units of ``rstd``), rounded from 32 bits and not from ``y``.
     ``keep=False`` leaves ``y`` out; ``save`` returns ``rstd`` for ``rms_norm_grad``.  Differentiable in ``x``, ``residual`` and ``weight`` through
-    ``y`` and ``residual``; the 8-bit form carries no gradient.
+    ``y`` and ``residual``, once; the 8-bit form carries no gradient.
     """
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
         if not keep:
             raise ValueError("gradients pass through y: keep=True")
         refuse_captured_gradients("rms_norm", "rms_norm_grad")
-        return NormResult(*_Norm.apply(x, weight, residual, float(eps), bool(quantize)))
+        return NormResult(*_ext().rms_norm_node(x, weight, residual, float(eps), bool(quantize)))
     return NormResult(*_ext().rms_norm(x, weight, residual, float(eps), bool(quantize), bool(keep), bool(save)))
 
 
@@ -47,23 +47,3 @@ def rms_norm_grad(grad_y: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, r
     """Gradients ``(grad_x, grad_weight)`` of ``rms_norm``; ``grad_x`` is that of ``residual`` as well.  ``h`` is what was normalised (the
     returned ``residual``, or ``x`` without one), ``grad_residual`` the gradient of the returned ``residual``.  Sums have one order on every run."""
     return _ext().rms_norm_grad(grad_y, h, weight, rstd, grad_residual)
-
-
-class _Norm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, residual, eps, quantize):
-        y, q, scales, stream, rstd = _ext().rms_norm(x, weight, residual, eps, quantize, True, True)
-        ctx.save_for_backward(x if stream is None else stream, weight, rstd)
-        ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(*(t for t in (q, scales, rstd) if t is not None))
-        return y, q, scales, stream, rstd
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_y, _q, _scales, grad_stream, _rstd):
-        refuse_captured_gradients("rms_norm", "rms_norm_grad")
-        if grad_y is None:
-            return grad_stream, None, grad_stream if ctx.needs_input_grad[2] else None, None, None
-        h, weight, rstd = ctx.saved_tensors
-        grad_x, grad_weight = _ext().rms_norm_grad(grad_y.contiguous(), h, weight, rstd, None if grad_stream is None else grad_stream.contiguous())
-        return grad_x, grad_weight, grad_x if ctx.needs_input_grad[2] else None, None, None

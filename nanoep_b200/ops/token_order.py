@@ -1,7 +1,7 @@
 """A batch sorted by expert and back on one GPU (csrc/token_order.cu): the local counterpart of dispatch and combine.
 
 No peer window, no host wait for counts and a fixed row order: forward calls can be captured in a CUDA graph, and rows, outputs
-and gate weights are differentiable.  ``slot`` is the row of one choice (token ``t``, choice ``k``); the rows of an expert are
+and gate weights are differentiable (once).  ``slot`` is the row of one choice (token ``t``, choice ``k``); the rows of an expert are
 ordered by (t, k).
 """
 
@@ -49,7 +49,7 @@ def sort_tokens(x: torch.Tensor, order: TokenOrder, *, scales: torch.Tensor | No
         if scales is not None:
             raise ValueError("rows that travel with scales have no gradient")
         refuse_captured_gradients("sort_tokens", "sort_tokens_grad")
-        return _Sort.apply(x, order.slots, order.slot_map, bool(zero_padding))
+        return _ext().sort_tokens_node(x, order.slots, order.slot_map, bool(zero_padding))
     rows, row_scales = _ext().sort_tokens(x, order.slots, order.slot_map, scales, bool(zero_padding))
     return rows if scales is None else (rows, row_scales)
 
@@ -62,7 +62,7 @@ def unsort_tokens(y: torch.Tensor, order: TokenOrder, weights: torch.Tensor | No
     """
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (y, weights, bias)):
         refuse_captured_gradients("unsort_tokens", "unsort_tokens_grad")
-        return _Unsort.apply(y, order.slots, order.slot_map, weights, bias)
+        return _ext().unsort_tokens_node(y, order.slots, order.slot_map, weights, bias)
     return _ext().unsort_tokens(y, order.slots, order.slot_map, weights, bias)
 
 
@@ -74,34 +74,3 @@ def sort_tokens_grad(grad_rows: torch.Tensor, order: TokenOrder) -> torch.Tensor
 def unsort_tokens_grad(grad_out: torch.Tensor, y: torch.Tensor, order: TokenOrder, weights: torch.Tensor | None = None):
     """Gradients of ``unsort_tokens`` in ``y`` (zero in rows without a choice) and in ``weights`` (0 for masked choices; ``None`` without)."""
     return _ext().unsort_tokens_grad(grad_out, y, order.slots, order.slot_map, weights)
-
-
-class _Sort(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, slots, slot_map, zero_padding):
-        ctx.save_for_backward(slots, slot_map)
-        return _ext().sort_tokens(x, slots, slot_map, None, zero_padding)[0]
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_rows):
-        refuse_captured_gradients("sort_tokens", "sort_tokens_grad")
-        return _ext().unsort_tokens(grad_rows.contiguous(), *ctx.saved_tensors, None, None), None, None, None
-
-
-class _Unsort(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, y, slots, slot_map, weights, bias):
-        ctx.save_for_backward(y, slots, slot_map, weights)
-        return _ext().unsort_tokens(y, slots, slot_map, weights, bias)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_out):
-        refuse_captured_gradients("unsort_tokens", "unsort_tokens_grad")
-        y, slots, slot_map, weights = ctx.saved_tensors
-        grad_out = grad_out.contiguous()
-        grad_y = grad_weights = None
-        if ctx.needs_input_grad[0] or ctx.needs_input_grad[3]:
-            grad_y, grad_weights = _ext().unsort_tokens_grad(grad_out, y, slots, slot_map, weights)
-        return grad_y, None, None, grad_weights, grad_out if ctx.needs_input_grad[4] else None

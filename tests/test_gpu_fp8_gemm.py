@@ -180,12 +180,18 @@ def test_many_units_and_experts():
 
 
 def test_a_row_does_not_depend_on_the_others():
-    """The same row alone, in a small and in a large expert, and under every hint: the same bits."""
+    """The same row alone, in a small and in a large expert, and under a hint: the order of the sums may differ with the tile, nothing else."""
     a, sa, w, sw, offsets, n, real = _problem([600], 1024, 256)
     whole = grouped_gemm_fp8(a, sa, w, sw, offsets)
     for first, last in ((0, 1), (5, 100), (128, 384), (599, 600)):
         part = grouped_gemm_fp8(a[first:last].contiguous(), sa[first:last].contiguous(), w, sw, torch.tensor([0, last - first], device="cuda"), max_expert_rows=last - first)
         torch.testing.assert_close(part.float(), whole[first:last].float(), rtol=2.0**-7, atol=1e-3)
+
+
+@pytest.mark.parametrize("rows,experts,most,k_blocks", [(1, 1, 1, 56), (64, 1, 0, 16), (512, 32, 32, 56), (512, 32, 0, 56), (4096, 32, 0, 16), (40000, 32, 0, 56), (7, 256, 0, 8), (3, 3, 900, 1)])
+def test_the_choice_covers_every_call(rows, experts, most, k_blocks):
+    tile, ctas = gg._ext().fp8_gemm_choice(rows, experts, most, 16, k_blocks, 148)
+    assert tile in (32, 64, 128) and ctas in (1, 2, 4, 8) and (tile < 128 or ctas == 1)
 
 
 def test_extreme_scales_and_values():

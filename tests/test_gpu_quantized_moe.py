@@ -103,6 +103,30 @@ def test_every_choice_masked():
     assert not out.any()
 
 
+def test_no_tokens():
+    layer = _layer(4, 256, 128)
+    out, stream = layer(torch.empty(0, 256, device="cuda", dtype=torch.bfloat16), torch.empty(0, 2, dtype=torch.int64, device="cuda"), torch.empty(0, 2, device="cuda"),
+                        residual=torch.empty(0, 256, device="cuda", dtype=torch.bfloat16))
+    assert out.shape == stream.shape == (0, 256)
+
+
+def test_two_layers_at_once():
+    """Two layers on two streams share no state."""
+    layers = [_layer(8, 512, 256), _layer(4, 1024, 128)]
+    batches = [_batch(200, h, e, 2, s) for s, (h, e) in enumerate(((512, 8), (1024, 4)))]
+    want = [layer(*batch) for layer, batch in zip(layers, batches)]
+    streams = [torch.cuda.Stream() for _ in layers]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for layer, batch, stream in zip(layers, batches, streams):
+            with torch.cuda.stream(stream):
+                got.append(layer(*batch))
+    torch.cuda.synchronize()
+    for i, out in enumerate(got):
+        assert torch.equal(out, want[i % 2])
+
+
 def test_captured_step():
     layer = _layer(8, 512, 256)
     x, idx, gate = _batch(64, 512, 8, 4)

@@ -182,6 +182,61 @@ def test_gradient_of_the_stream_alone_and_without_rows():
     assert got.q.shape == (0, 64) and got.scales.shape == (0, 1) and dx.shape == (0, 64) and not dw.any()
 
 
+def test_differentiable_once():
+    x = torch.randn(2, 64, device="cuda", requires_grad=True)
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    with pytest.raises(RuntimeError, match="create_graph"):
+        torch.autograd.grad(rms_norm(x, w).y.sum(), x, create_graph=True)
+    total = (rms_norm(x, w).y * 2).sum() + (x * x).sum()
+    total.backward()
+    assert x.grad.isfinite().all() and w.grad.isfinite().all()
+
+
+def test_captured_forward_and_explicit_gradients():
+    x, r, g = (torch.randn(40, 512, device="cuda").to(torch.bfloat16) for _ in range(3))
+    w = torch.rand(512, device="cuda").to(torch.bfloat16)
+
+    def step():
+        got = rms_norm(x, w, residual=r, quantize=True, save=True)
+        return (got.y, got.q.view(torch.uint8), got.scales, got.residual, *rms_norm_grad(g, got.residual, w, got.rstd, grad_residual=g))
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+        with pytest.raises(RuntimeError, match="rms_norm_grad"):
+            rms_norm(x.detach().requires_grad_(), w)
+    for _ in range(2):
+        for t in (x, r, g):
+            t.normal_()
+        graph.replay()
+        for a, b in zip(held, step()):
+            assert torch.equal(a, b)
+
+
+def test_a_batch_on_another_stream():
+    """A long queue on one stream and the call on another: ordered by the caller, and the outputs belong to the call's stream."""
+    stream = torch.cuda.Stream()
+    x = torch.randn(64, 4096, device="cuda")
+    w = torch.ones(4096, device="cuda")
+    want = rms_norm(x, w, quantize=True)
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        got = [rms_norm(x, w, quantize=True) for _ in range(20)]
+    torch.cuda.current_stream().wait_stream(stream)
+    for g in got:
+        assert torch.equal(g.y, want.y) and torch.equal(g.scales, want.scales) and torch.equal(g.q.view(torch.uint8), want.q.view(torch.uint8))
+
+
+def test_largest_values_of_the_type():
+    """h * weight near the largest 32-bit value: neither the quotient nor the scale's product overflows where the result does not."""
+    x = torch.full((1, 256), 2.0**126, device="cuda")
+    x[0, 1::2] = 2.0**120
+    q, scales = quantize_rows(x)
+    assert torch.equal(q.float()[0, :2], torch.tensor([448.0, 7.0], device="cuda"))
+    torch.testing.assert_close(q.double() * scales.double().repeat_interleave(128, 1), x.double(), rtol=2.0**-20, atol=0)
+
+
 def test_refusals():
     x = torch.randn(2, 64, device="cuda")
     w = torch.ones(64, device="cuda")

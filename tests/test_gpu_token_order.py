@@ -173,6 +173,21 @@ def test_gradients_against_differences():
         assert abs(float(slope - (grad.double() * d.double()).sum())) <= 64 * 2.0**-24 * float(size) + 2.0**-20 * float((grad * d).abs().sum())
 
 
+def test_gradients_of_some_inputs_and_once():
+    order = plan_tokens(_routing(9, 4, 2, "uniform").cuda(), 4)
+    y, w, b, g = torch.randn(order.capacity, 32, device="cuda"), torch.rand(9, 2, device="cuda"), torch.randn(9, 32, device="cuda"), torch.randn(9, 32, device="cuda")
+    full = unsort_tokens_grad(g, y, order, w)
+    for wanted in ((0,), (1,), (2,), (0, 2), (1, 2)):
+        leaves = [t.clone().requires_grad_(i in wanted) for i, t in enumerate((y, w, b))]
+        out = unsort_tokens(leaves[0], order, leaves[1], bias=leaves[2])
+        for i, grad in zip(wanted, torch.autograd.grad(out, [leaves[i] for i in wanted], g)):
+            assert torch.equal(grad, (*full, g)[i])
+    x = torch.randn(9, 32, device="cuda", requires_grad=True)
+    for out in (sort_tokens(x, order).sum(), unsort_tokens(y.clone().requires_grad_() * 1, order).sum()):
+        with pytest.raises(RuntimeError, match="create_graph"):
+            out.backward(create_graph=True)
+
+
 def test_an_expert_id_out_of_range_is_masked_and_reported():
     idx = torch.tensor([[0, 5], [7, 1], [-2, 2]], device="cuda")
     order = plan_tokens(idx, 4)
