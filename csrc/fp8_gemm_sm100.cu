@@ -4,18 +4,26 @@
 //
 // plain (times a factor per row) or silu(gate) * up, to bf16 or to e4m3 with a scale for each 128 output columns.
 //
-// The scales are any 32-bit values, so the tensor cores sum one block of 128 at a time into TMEM and the epilogue warps add it, scaled,
-// to sums that stay in their registers.  Rows are the M operand: a thread owns a row, its scale is one register, and a block
-// costs it one multiply-add per column (with the rows as N every column would need a scale of its own from shared memory, 4 cycles a
-// load for 4 columns: twice the tensor cores' time).
+// The scales are any 32-bit values, so the tensor cores sum one block of 128 columns at a time into TMEM and the epilogue warps add it, scaled,
+// to sums that stay in their registers.  Rows are the M operand: a thread owns a row, its scale is one register, and a block costs it
+// one multiply-add per column.  (Experts of few rows: fp8_gemm_few_sm100.cu.)
 //
-// A cluster of two CTAs computes 256 rows x 256 weight rows (tcgen05.mma.cta_group::2): each CTA loads its own 128 rows and half of the
-// weight rows by TMA, the leader issues the MMAs, each CTA's TMEM holds its rows' block sums, two buffers of 256 columns, so that
-// the MMAs of a block run under the multiply-adds of the one before.  With SwiGLU the 256 weight rows are 64 gate rows, their 64 up rows
-// and again 64 of each, which puts both factors of an output into the same thread.
+// A CTA computes 128 rows x 256 weight rows (tcgen05.mma, N = 256) with two block sums of 256 columns in TMEM, so that the MMAs of a block run
+// under the multiply-adds of the one before.  With SwiGLU the weight rows are 64 gate rows, their 64 up rows and again 64 of each, which puts
+// both factors of an output into the same thread.
 //
-// All waits are bounded; on expiry a CTA records a code in `status`, stops issuing work, and both CTAs still meet at the
-// final cluster barrier and free their TMEM.
+// What bounds it.  Experts up to 128 rows: the weights' way from memory (32 experts of 7168 x 2048: 64 rows each up 174 us = 5.4 TB/s, down 99 us).  More: a
+// block of 128 columns, 512 cycles of MMA, takes 0.64 to 0.70 us.  0.37 us of that are the operands' way (48 KB, 68 bytes a cycle), 0.48 us that
+// and the MMAs, which read 48 KB of the same shared memory, and the rest that an epilogue warp gets through 128 columns in 0.6 us:
+// under this traffic a load from shared memory or a look at a barrier takes 200 to 300 cycles.  Hence: no fence where a value read says
+// enough, scales and the next block's state asked for a block ahead, the tile's description left by the warp that loads the scales.
+// In a long run the power limit (1000 W, 1.6 GHz): 32 x (1024 +- 32) rows up 1325 us = 1.45 PFLOP/s of real rows, down 650 us.
+//
+// Tried: pairs of CTAs (cta_group::2, 256 rows, two thirds of the operand traffic): 0.69 us a block as well, with a signal between the CTAs in every
+// block; at 128 rows an expert half of a pair is idle (up 257 us instead of 188).  Two columns per instruction (fma.rn.f32x2): no faster, and
+// the pairs need registers.  Scales by plain loads: 0.6 us a block more.  32 columns twice in flight: registers spill.
+//
+// All waits are bounded; on expiry a CTA records a code in `status`, stops issuing work, waits for its own copies and frees its TMEM.
 #include "fp8_gemm_sm100.hpp"
 
 #include "fp8_prim.cuh"
