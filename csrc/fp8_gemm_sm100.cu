@@ -45,8 +45,8 @@ constexpr int kStageBytes = kRowBytes + kWeightBytes;
 constexpr int kStages = 3;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 128 + 32 * kEpiWarps;   // a warpgroup that loads and issues, two that add up
-// A launch of 384 threads gives each 168 registers.  The sums need more: 72 + 2 * 208 < 3 * 168, what the block was launched with.
-constexpr int kFewRegisters = 72, kManyRegisters = 208;
+// A launch of 384 threads gives each 168 registers.  The sums need more: 56 + 2 * 224 = 3 * 168, what the block was launched with.
+constexpr int kFewRegisters = 56, kManyRegisters = 224;
 static_assert(128 * kFewRegisters + 32 * kEpiWarps * kManyRegisters <= kThreads * 168, "registers of the launch");
 constexpr int kTmemCols = 512;
 constexpr int kPiecePitch = 256 + 16;            // a thread's part of an output row on its way out: 8 rows hit all banks once
@@ -99,13 +99,6 @@ __device__ __forceinline__ Tile locate_warp(const Shared& sh, const Args& args, 
     return tile_of(sh, args, unit, lo);
 }
 
-// 16 consecutive fp32 columns of this thread's TMEM lane
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-                 : "r"(taddr));
-}
 // A row's piece leaves by a copy of its thread's own: whole sectors, and nothing waits for them but the piece's next use.
 __device__ __forceinline__ void send_piece(void* dst, const void* piece, int bytes) {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -270,22 +263,16 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
             for (int kb0 = 0; kb0 < k_blocks; kb0 += kScaleBlocks, ++chunk) {
                 const float w = kb0 + (lane >> 1) < k_blocks && lane < 2 * kScaleBlocks ? sw[kb0 + (lane >> 1)] : 0.f;
                 const int slot = chunk & 1;
+                for (int i = 0; i < 4; ++i) {  // a row a lane at a time, for want of registers
+                    const int r = i * 32 + lane;
+                    const float* sa = args.a_scales + (int64_t(t.row0) + r) * k_blocks + kb0;
+                    float v[kScaleBlocks];
 #pragma unroll
-                for (int i = 0; i < 4; i += 2) {  // two rows a lane at a time, for want of registers
-                    float v[2][kScaleBlocks];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int r = (i + h) * 32 + lane;
-                        const float* sa = args.a_scales + (int64_t(t.row0) + r) * k_blocks + kb0;
-#pragma unroll
-                        for (int j = 0; j < kScaleBlocks; ++j) v[h][j] = r < t.rows && kb0 + j < k_blocks ? sa[j] : 0.f;
-                    }
+                    for (int j = 0; j < kScaleBlocks; ++j) v[j] = r < t.rows && kb0 + j < k_blocks ? sa[j] : 0.f;
                     if (i == 0) ok = __all_sync(0xffffffffu, wait_block(&sh.scale_empty[slot], (uint32_t(chunk >> 1) & 1u) ^ 1u, limit_ns, abort_flag));
                     if (!ok) break;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int j = 0; j < kScaleBlocks; ++j) sh.row_scales[slot][j][(i + h) * 32 + lane] = v[h][j];
+                    for (int j = 0; j < kScaleBlocks; ++j) sh.row_scales[slot][j][r] = v[j];
                 }
                 if (!ok) {
                     if (lane == 0) fail(kPipeTimeout);
@@ -345,10 +332,10 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                     ++chunk;
                 }
             };
-            // A block is 16, 32, 16, 32, 16 and 16 columns, the next ones on their way while these are added; the first of a block under the last
-            // of the one before, where it is complete by then.  (One after the other a block took 1070 cycles, mostly latencies.)
+            // 64 columns at a time, two loads of 32 in flight while the two before are added; a block's first ones under the last of the block before,
+            // where it is complete by then.  A wait for loads is a wait for all of them, about 130 cycles under the MMAs: two a block.
             const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(group * 128);
-            uint32_t a[32], b[16];
+            uint32_t a[32], b[32];
             fetch_scales(0);
             use_scales(0);
             bool begun = false;  // the loads of the block's first columns have been issued
@@ -361,7 +348,10 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                         break;
                     }
                     tc_fence_after();
-                    if (any) tmem_ld16(taddr + uint32_t(buf * kTileCols), b);
+                    if (any) {
+                        tmem_ld32(taddr + uint32_t(buf * kTileCols), a);
+                        tmem_ld32(taddr + uint32_t(buf * kTileCols) + 32, b);
+                    }
                 }
                 if (++stage == kStages) {
                     stage = 0;
@@ -370,41 +360,27 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                 if (any) {
                     const uint32_t at = taddr + uint32_t(buf * kTileCols);
                     const float g0 = f0, g1 = kSwiGLU ? f1 : f0;
-                    auto add_a = [&](int c, int columns) {
+                    auto add = [&](const uint32_t (&v)[32], int c) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (j < columns) acc[c + j] = fmaf(__uint_as_float(a[j]), c < 64 ? g0 : g1, acc[c + j]);
-                    };
-                    auto add_b = [&](int c) {
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) acc[c + j] = fmaf(__uint_as_float(b[j]), c < 64 ? g0 : g1, acc[c + j]);
+                        for (int j = 0; j < 32; ++j) acc[c + j] = fmaf(__uint_as_float(v[j]), c < 64 ? g0 : g1, acc[c + j]);
                     };
                     tmem_ld_wait();
-                    tmem_ld32(at + 16, a);
                     if (kb + 1 < k_blocks) fetch_scales(kb + 1);
-                    add_b(0);
-                    tmem_ld_wait();
-                    tmem_ld16(at + 48, b);
-                    add_a(16, 32);
-                    tmem_ld_wait();
+                    add(a, 0);
                     tmem_ld32(at + 64, a);
-                    add_b(48);
-                    tmem_ld_wait();
-                    tmem_ld16(at + 96, b);
+                    add(b, 32);
+                    tmem_ld32(at + 96, b);
                     const bool next_done = block_done(&sh.done[stage], phase);
-                    add_a(64, 32);
-                    tmem_ld_wait();
-                    tmem_ld16(at + 112, a);
-                    add_b(96);
                     tmem_ld_wait();
                     tc_fence_before();
                     if (lane == 0) arrive_read(empty_addr + uint32_t(buf) * 8u);
                     begun = __all_sync(0xffffffffu, kb + 1 < k_blocks && next_done);
-                    if (begun) {
-                        tc_fence_after();
-                        tmem_ld16(taddr + uint32_t((buf ^ 1) * kTileCols), b);
-                    }
-                    add_a(112, 16);
+                    if (begun) tc_fence_after();
+                    const uint32_t next = taddr + uint32_t((buf ^ 1) * kTileCols);
+                    add(a, 64);
+                    if (begun) tmem_ld32(next, a);
+                    add(b, 96);
+                    if (begun) tmem_ld32(next + 32, b);
                 } else {
                     tc_fence_before();
                     if (lane == 0) arrive_read(empty_addr + uint32_t(buf) * 8u);
