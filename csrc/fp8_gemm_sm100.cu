@@ -226,26 +226,29 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
         if (elect_one()) {
             int stage = 0, block = 0;
             uint32_t phase = 0;
+            bool loaded = false;  // as of the block before: a look at a barrier takes 190 cycles, under the MMAs none
             for (int unit = int(blockIdx.x); unit < units && !*abort_flag; unit += int(gridDim.x)) {
                 for (int kb = 0; kb < k_blocks; ++kb, ++block) {
-                    const int buf = block & 1;
-                    if (!wait_block(&sh.full[stage], phase, limit_ns, abort_flag) || !wait_block(&sh.tmem_empty[buf], (uint32_t(block >> 1) & 1u) ^ 1u, limit_ns, abort_flag)) {
+                    const int buf = block & 1, s = stage;
+                    if ((!loaded && !wait_block(&sh.full[stage], phase, limit_ns, abort_flag)) ||
+                        !wait_block(&sh.tmem_empty[buf], (uint32_t(block >> 1) & 1u) ^ 1u, limit_ns, abort_flag)) {
                         fail(kPipeTimeout);
                         break;
                     }
                     tc_fence_after();
-                    const uint8_t* tile = smem + stage * kStageBytes;
+                    if (++stage == kStages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                    loaded = block_done(&sh.full[stage], phase);
+                    const uint8_t* tile = smem + s * kStageBytes;
                     const uint64_t a_desc = smem_desc_sw128(tile), b_desc = smem_desc_sw128(tile + kRowBytes);
 #pragma unroll
                     for (int k = 0; k < 4; ++k)  // 32 values = 32 bytes inside the 128-byte swizzle row
                         mma_e4m3(tmem_base + uint32_t(buf * kTileCols), a_desc + uint64_t(k * 2), b_desc + uint64_t(k * 2), kInstrDesc, k != 0 ? 1u : 0u);
                     // One barrier per stage tells both the producer and the epilogue.  The epilogue has seen a block before the stage's next one can
                     // be done: that one waits for its TMEM columns.
-                    tc_commit(&sh.done[stage]);
-                    if (++stage == kStages) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
+                    tc_commit(&sh.done[s]);
                 }
             }
         }
