@@ -137,6 +137,7 @@ std::pair<at::Tensor, at::Tensor> rms_norm_grad(const at::Tensor& grad_y, const 
     a.weight_f32 = weight.scalar_type() == at::kFloat;
     a.aligned = a.hidden % 8 == 0 && on16(a.grad_y) && on16(a.h) && on16(a.weight) && on16(grad_stream);
     launched(norm::launch_norm_grad(a, norm::Type(type), sms, c10::cuda::getCurrentCUDAStream()), "rms_norm_grad");
+    PeerWindow::launches += 1;  // and the sum of the blocks' parts
     return {grad_x, grad_weight};
 }
 

@@ -10,7 +10,7 @@
 
 namespace nep {
 
-int64_t PeerWindow::launches = 0;
+std::atomic<int64_t> PeerWindow::launches{0};
 int64_t PeerWindow::queued_ahead = 0;
 
 namespace {

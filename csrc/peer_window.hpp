@@ -6,6 +6,7 @@
 // device trap; a window can also adopt other windows of the same process as "logical peers" so a
 // whole group runs on one GPU; operation parities select between the two copies of each region.
 #pragma once
+#include <atomic>
 #include <cstdint>
 #include <string>
 #include <utility>
@@ -85,7 +86,7 @@ public:
     void order_after_last(cudaStream_t stream);
 
     // Launch counter for diagnostics and benchmarks.
-    static int64_t launches;
+    static std::atomic<int64_t> launches;  // gradients are queued by autograd's threads as well
     static int64_t queued_ahead;  // dispatches whose followers were queued before the host had the counts
 
 private:
