@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(256) unsort_kernel(const UnsortArgs a, int pie
 // A block per token: its gradient row stays in the SM's first cache while every choice's row is read, multiplied and written.
 template <typename T, bool kAligned>
 __global__ void __launch_bounds__(256) unsort_grad_kernel(const UnsortGradArgs a) {
-    __shared__ float part[8][kMaxTopk];
+    __shared__ double part[8][kMaxTopk];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (int64_t(blockIdx.x) >= a.tokens) {  // rows without a choice
         const int64_t s0 = (int64_t(blockIdx.x) - a.tokens) * 8 * kZeroRows + warp * kZeroRows;
@@ -336,7 +336,7 @@ __global__ void __launch_bounds__(256) unsort_grad_kernel(const UnsortGradArgs a
     const T* g_row = static_cast<const T*>(a.grad_out) + t * a.hidden;
     for (int k = 0; k < a.topk; ++k) {
         const int slot = a.slots[t * a.topk + k];
-        float dot = 0.f;
+        double dot = 0.0;  // of eight products in 32 bits at a time: the sum may be far smaller than its terms
         if (uint32_t(slot) < uint64_t(a.capacity)) {
             const float w = a.weights != nullptr ? a.weights[t * a.topk + k] : 1.f;
             const T* y_row = static_cast<const T*>(a.y) + int64_t(slot) * a.hidden;
@@ -345,23 +345,26 @@ __global__ void __launch_bounds__(256) unsort_grad_kernel(const UnsortGradArgs a
                 load8<T, kAligned>(g_row, c, a.hidden, g);
                 if (a.grad_weights != nullptr) {
                     load8<T, kAligned>(y_row, c, a.hidden, y);
+                    float eight = 0.f;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) dot += g[j] * y[j];
+                    for (int j = 0; j < 8; ++j) eight += g[j] * y[j];
+                    dot += double(eight);
                 }
 #pragma unroll
                 for (int j = 0; j < 8; ++j) g[j] *= w;
                 store8<T, kAligned>(static_cast<T*>(a.grad_y) + int64_t(slot) * a.hidden, c, a.hidden, g);
             }
         }
-        dot = warp_sum(dot);
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
         if (lane == 0) part[warp][k] = dot;
     }
     __syncthreads();
     if (a.grad_weights != nullptr && threadIdx.x < a.topk) {
-        float s = 0.f;
+        double s = 0.0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) s += part[i][threadIdx.x];
-        a.grad_weights[t * a.topk + threadIdx.x] = s;
+        a.grad_weights[t * a.topk + threadIdx.x] = float(s);
     }
 }
 
