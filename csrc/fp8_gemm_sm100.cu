@@ -299,14 +299,27 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
         int block = 0, stage = 0, chunk = 0, exchanges = 0;
         uint32_t phase = 0;
         bool ok = true;
-        for (int unit = int(blockIdx.x); unit < units && ok; unit += int(gridDim.x)) {
-            // the warp that loads the scales knows the tile already
-            ok = __all_sync(0xffffffffu, wait_block(&sh.scale_full[chunk & 1], uint32_t(chunk >> 1) & 1u, limit_ns, abort_flag));
-            if (!ok) {
-                if (lane == 0) fail(kPipeTimeout);
-                break;
+        // Under the MMAs' operand traffic an access to shared memory takes 200 to 300 cycles, a look at a barrier as well: scales and the state of
+        // the next block are asked for while a block is added, the next tile's while a tile leaves, and used behind it.
+        float sr = 0.f, sw0 = 0.f, sw1 = 0.f;
+        auto fetch_scales = [&](int kb) {
+            const int at = kb % kScaleBlocks, slot = chunk & 1;
+            if (at == 0) {
+                ok = __all_sync(0xffffffffu, wait_block(&sh.scale_full[slot], uint32_t(chunk >> 1) & 1u, limit_ns, abort_flag)) && ok;
+                if (!ok && lane == 0) fail(kPipeTimeout);
             }
-            const int4 told = sh.tile[chunk & 1];
+            sr = sh.row_scales[slot][at][r];
+            sw0 = sh.weight_scales[slot][at][kSwiGLU ? 0 : group];
+            if (kSwiGLU) sw1 = sh.weight_scales[slot][at][1];
+        };
+        int4 told = make_int4(0, 0, 0, 0);  // the tile: the warp that loads the scales knows it
+        auto fetch_tile = [&]() {
+            fetch_scales(0);
+            told = sh.tile[chunk & 1];
+        };
+        if (!kSwiGLU && int(blockIdx.x) < units) fetch_tile();
+        for (int unit = int(blockIdx.x); unit < units && ok; unit += int(gridDim.x)) {
+            if (kSwiGLU) fetch_tile();  // no registers for it ahead
             const Tile t{told.x, told.y, told.z, told.w};
             const bool real = r < t.rows;
             const bool any = quarter * 32 < t.rows;  // of this warp's rows
@@ -316,16 +329,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
             float acc[128];
 #pragma unroll
             for (int j = 0; j < 128; ++j) acc[j] = 0.f;
-            // Under the MMAs' operand traffic an access to shared memory takes 200 to 300 cycles, a look at a barrier as well: scales and the state of
-            // the next block are asked for while a block is added, and used behind it.
-            float sr = 0.f, sw0 = 0.f, sw1 = 0.f, f0 = 0.f, f1 = 0.f;
-            auto fetch_scales = [&](int kb) {
-                const int at = kb % kScaleBlocks, slot = chunk & 1;
-                if (at == 0) ok = __all_sync(0xffffffffu, wait_block(&sh.scale_full[slot], uint32_t(chunk >> 1) & 1u, limit_ns, abort_flag)) && ok;
-                sr = sh.row_scales[slot][at][r];
-                sw0 = sh.weight_scales[slot][at][kSwiGLU ? 0 : group];
-                if (kSwiGLU) sw1 = sh.weight_scales[slot][at][1];
-            };
+            float f0 = 0.f, f1 = 0.f;
             auto use_scales = [&](int kb) {
                 f0 = sr * sw0;
                 if (kSwiGLU) f1 = sr * sw1;
@@ -339,8 +343,9 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
             // where it is complete by then.  A wait for loads is a wait for all of them, about 130 cycles under the MMAs: two a block.
             const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(group * 128);
             uint32_t a[32], b[32];
-            fetch_scales(0);
             use_scales(0);
+            float out_scale = 1.f;  // asked for ahead as well
+            if (!kSwiGLU && args.row_scale != nullptr && real) out_scale = args.row_scale[row];
             bool begun = false;  // the loads of the block's first columns have been issued
             for (int kb = 0; kb < k_blocks; ++kb, ++block) {
                 const int buf = block & 1;
@@ -392,6 +397,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                 if (kb + 1 < k_blocks) use_scales(kb + 1);
             }
             if (!ok) break;
+            if (!kSwiGLU && unit + int(gridDim.x) < units) fetch_tile();
             if (!any) continue;
             constexpr int kCols = kSwiGLU ? 64 : 128;  // output columns of this thread
             pieces_read();                             // the tile before, long past
@@ -400,9 +406,8 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
 #pragma unroll
                 for (int j = 0; j < 64; ++j) acc[j] = __fdividef(acc[j], 1.f + __expf(-acc[j])) * acc[64 + j];
             } else if (args.row_scale != nullptr) {
-                const float f = real ? args.row_scale[row] : 0.f;
 #pragma unroll
-                for (int j = 0; j < 128; ++j) acc[j] *= f;
+                for (int j = 0; j < 128; ++j) acc[j] *= out_scale;
             }
             if (kQuantize) {
                 float m = 0.f;
