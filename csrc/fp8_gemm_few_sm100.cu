@@ -37,23 +37,25 @@ using namespace gemm::tc;
 using namespace rows;
 
 constexpr int kLanes = 128;                    // weight rows of one accumulator
-constexpr int kWeightBytes = 2 * kLanes * 128; // of a stage: two accumulators' rows, 128 columns
+constexpr int kLanesBytes = kLanes * 128;      // an accumulator's rows of a stage, 128 columns
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 128 + 32 * kEpiWarps;
 constexpr int kTmemCols = 512;
 constexpr int kSlice = 32;                     // rows exchanged at a time, half of them from each epilogue group
 
-template <int kTileRows>
+// One accumulator (128 output columns a tile) or two.
+template <int kAcc, int kTileRows>
 struct Shape {
+    static constexpr int kWeightBytes = kAcc * kLanesBytes;
     static constexpr int kStageBytes = kWeightBytes + kTileRows * 128;
-    static constexpr int kStages = kTileRows <= 32 ? 5 : 4;
-    static constexpr int kBufs = kTmemCols / (2 * kTileRows) < 8 ? kTmemCols / (2 * kTileRows) : 8;
+    static constexpr int kStages = kAcc == 1 ? 8 : kTileRows <= 32 ? 5 : 4;
+    static constexpr int kBufs = kTmemCols / (kAcc * kTileRows) < 8 ? kTmemCols / (kAcc * kTileRows) : 8;
 };
 
-template <int kTileRows>
+template <int kAcc, int kTileRows>
 struct Shared {
-    using S = Shape<kTileRows>;
-    float parts[kSlice * 2 * kLanes];  // [source CTA][row][accumulator][lane]
+    using S = Shape<kAcc, kTileRows>;
+    float parts[kSlice * kAcc * kLanes];  // [source CTA][row][accumulator][lane]
     float row_scales[2][kScaleBlocks][kTileRows];
     float weight_scales[2][kScaleBlocks][2];
     uint64_t full[S::kStages], empty[S::kStages], tmem_full[S::kBufs], tmem_empty[S::kBufs];
@@ -64,11 +66,11 @@ struct Shared {
     int rows[kMaxExperts];
     int first_tile[kMaxExperts + 1];
 };
-template <int kTileRows>
+template <int kAcc, int kTileRows>
 constexpr size_t smem_bytes() {
-    return size_t(Shape<kTileRows>::kStages) * Shape<kTileRows>::kStageBytes + sizeof(Shared<kTileRows>);
+    return size_t(Shape<kAcc, kTileRows>::kStages) * Shape<kAcc, kTileRows>::kStageBytes + sizeof(Shared<kAcc, kTileRows>);
 }
-static_assert(smem_bytes<32>() <= 232448 && smem_bytes<64>() <= 232448, "shared memory of a CTA");
+static_assert(smem_bytes<2, 32>() <= 232448 && smem_bytes<2, 64>() <= 232448 && smem_bytes<1, 32>() <= 232448 && smem_bytes<1, 64>() <= 232448, "shared memory of a CTA");
 
 struct Tile {
     int expert, row0, rows, nt;
@@ -78,8 +80,8 @@ __device__ __forceinline__ int tile_rows(int n, int largest) {
     const int tiles = (n + largest - 1) / largest;
     return ((n + tiles - 1) / tiles + 15) & ~15;
 }
-template <int kTileRows>
-__device__ __forceinline__ Tile locate(const Shared<kTileRows>& sh, int experts, int n_tiles, int unit) {
+template <int kAcc, int kTileRows>
+__device__ __forceinline__ Tile locate(const Shared<kAcc, kTileRows>& sh, int experts, int n_tiles, int unit) {
     const int at = unit / n_tiles;
     int lo = 0, hi = experts;  // first_tile[lo] <= at < first_tile[hi]
     while (hi - lo > 1) {
@@ -119,12 +121,13 @@ __device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, uin
     }
 }
 
-template <bool kSwiGLU, bool kQuantize, int kTileRows>
+template <int kAcc, bool kSwiGLU, bool kQuantize, int kTileRows>
 __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_few_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args args, const int ctas) {
-    using P = Shape<kTileRows>;
+    static_assert(kAcc == 2 || !kSwiGLU, "gate and up rows");
+    using P = Shape<kAcc, kTileRows>;
     constexpr int kStages = P::kStages, kBufs = P::kBufs;
     extern __shared__ __align__(1024) uint8_t smem[];
-    Shared<kTileRows>& sh = *reinterpret_cast<Shared<kTileRows>*>(smem + kStages * P::kStageBytes);
+    Shared<kAcc, kTileRows>& sh = *reinterpret_cast<Shared<kAcc, kTileRows>*>(smem + kStages * P::kStageBytes);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int cta = int(cluster_ctarank());
     const uint64_t limit_ns = args.timeout_ns;
@@ -207,17 +210,17 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_few_kernel(const __grid_
                         break;
                     }
                     uint8_t* dst = smem + stage * P::kStageBytes;
-                    mbar_expect_tx(&sh.full[stage], uint32_t(kWeightBytes + n * 128));
+                    mbar_expect_tx(&sh.full[stage], uint32_t(P::kWeightBytes + n * 128));
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
-                        tma_load_3d(dst + i * kLanes * 128, &maps.weights, kb * 128, kSwiGLU ? t.nt * kLanes : (2 * t.nt + i) * kLanes,
+                    for (int i = 0; i < kAcc; ++i)
+                        tma_load_3d(dst + i * kLanesBytes, &maps.weights, kb * 128, kSwiGLU ? t.nt * kLanes : (kAcc * t.nt + i) * kLanes,
                                     kSwiGLU ? 2 * t.expert + i : t.expert, &sh.full[stage]);
                     int at = 0;  // boxes of 128, 64, 32 and 16 rows make up any multiple of 16
 #pragma unroll
                     for (int b = 0; b < 4; ++b) {
                         const int box = 128 >> b;
                         if (n & box) {
-                            tma_load_2d(dst + kWeightBytes + at * 128, &maps.rows[b], kb * 128, t.row0 + at, &sh.full[stage]);
+                            tma_load_2d(dst + P::kWeightBytes + at * 128, &maps.rows[b], kb * 128, t.row0 + at, &sh.full[stage]);
                             at += box;
                         }
                     }
@@ -247,13 +250,13 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_few_kernel(const __grid_
                     }
                     tc_fence_after();
                     const uint8_t* tile = smem + stage * P::kStageBytes;
-                    const uint64_t r_desc = smem_desc_sw128(tile + kWeightBytes);
+                    const uint64_t r_desc = smem_desc_sw128(tile + P::kWeightBytes);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint64_t w_desc = smem_desc_sw128(tile + i * kLanes * 128);
+                    for (int i = 0; i < kAcc; ++i) {
+                        const uint64_t w_desc = smem_desc_sw128(tile + i * kLanesBytes);
 #pragma unroll
                         for (int k = 0; k < 4; ++k)  // 32 values = 32 bytes inside the 128-byte swizzle row
-                            mma_e4m3(tmem_base + uint32_t((2 * buf + i) * kTileRows), w_desc + uint64_t(k * 2), r_desc + uint64_t(k * 2), idesc, k != 0 ? 1u : 0u);
+                            mma_e4m3(tmem_base + uint32_t((kAcc * buf + i) * kTileRows), w_desc + uint64_t(k * 2), r_desc + uint64_t(k * 2), idesc, k != 0 ? 1u : 0u);
                     }
                     tc_commit(&sh.empty[stage]);
                     tc_commit(&sh.tmem_full[buf]);
@@ -275,7 +278,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_few_kernel(const __grid_
         bool ok = true;
         for (int unit = cluster_id; unit < units && ok; unit += num_clusters) {
             const Tile t = locate(sh, args.experts, args.n_tiles, unit);
-            const int half = lane & 1, block = kSwiGLU ? half * args.n_blocks + t.nt : min(2 * t.nt + half, args.n_blocks - 1);
+            const int half = lane & 1, block = kSwiGLU ? half * args.n_blocks + t.nt : min(kAcc * t.nt + half % kAcc, args.n_blocks - 1);
             const float* sw = args.w_scales + (int64_t(t.expert) * kHalves * args.n_blocks + block) * args.k_blocks;
             for (int kb0 = k_first; kb0 < k_last; kb0 += kScaleBlocks, ++chunk) {
                 const int slot = chunk & 1;
@@ -314,9 +317,9 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_few_kernel(const __grid_
         for (int unit = cluster_id; unit < units && ok; unit += num_clusters) {
             const Tile t = locate(sh, args.experts, args.n_tiles, unit);
             const int half = ((t.rows + 15) & ~15) / 2;  // rows of a group, a multiple of 8
-            uint64_t sum[2][kCols / 2];
+            uint64_t sum[kAcc][kCols / 2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < kAcc; ++i)
 #pragma unroll
                 for (int j = 0; j < kCols / 2; ++j) sum[i][j] = 0;
             for (int kb = k_first; kb < k_last; ++kb) {
@@ -328,23 +331,24 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_few_kernel(const __grid_
                     break;
                 }
                 tc_fence_after();
-                const uint64_t w0 = pair_of(sh.weight_scales[slot][at][0]), w1 = pair_of(sh.weight_scales[slot][at][1]);
+                uint64_t w[kAcc];
+#pragma unroll
+                for (int i = 0; i < kAcc; ++i) w[i] = pair_of(sh.weight_scales[slot][at][i]);
                 const float* scales = &sh.row_scales[slot][at][group * half];
-                const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(2 * buf * kTileRows + group * half);
+                const uint32_t taddr = tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(kAcc * buf * kTileRows + group * half);
 #pragma unroll
                 for (int c = 0; c < kCols / 8; ++c) {
                     if (c * 8 >= half) break;
-                    uint32_t v[2][8];
-                    tmem_ld8(taddr + c * 8, v[0]);
-                    tmem_ld8(taddr + kTileRows + c * 8, v[1]);
+                    uint32_t v[kAcc][8];
+#pragma unroll
+                    for (int i = 0; i < kAcc; ++i) tmem_ld8(taddr + i * kTileRows + c * 8, v[i]);
                     const ulonglong2 s0 = *reinterpret_cast<const ulonglong2*>(scales + c * 8), s1 = *reinterpret_cast<const ulonglong2*>(scales + c * 8 + 4);
                     const uint64_t s[4] = {s0.x, s0.y, s1.x, s1.y};
                     tmem_ld_wait();
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        fma_pair(sum[0][c * 4 + j], v[0][2 * j], v[0][2 * j + 1], mul_pair(s[j], w0));
-                        fma_pair(sum[1][c * 4 + j], v[1][2 * j], v[1][2 * j + 1], mul_pair(s[j], w1));
-                    }
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int i = 0; i < kAcc; ++i) fma_pair(sum[i][c * 4 + j], v[i][2 * j], v[i][2 * j + 1], mul_pair(s[j], w[i]));
                 }
                 tc_fence_before();
                 __syncwarp();
@@ -374,9 +378,9 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_few_kernel(const __grid_
                 for (int j = 0; j < 16; ++j) {
                     if (s * 16 + j >= kCols || j >= each) break;
                     const int q = group * each + j, to = q / share;
-                    const uint32_t dst = map_to_cta(smem_u32(&sh.parts[((cta * share + q % share) * 2) * kLanes + feature]), uint32_t(to));
+                    const uint32_t dst = map_to_cta(smem_u32(&sh.parts[(cta * share + q % share) * kAcc * kLanes + feature]), uint32_t(to));
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
+                    for (int i = 0; i < kAcc; ++i) {
                         const uint64_t p = sum[i][(s * 16 + j) / 2];
                         st_cluster_f32(dst + i * kLanes * 4, __uint_as_float(j & 1 ? uint32_t(p >> 32) : uint32_t(p)));
                     }
@@ -392,25 +396,27 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_few_kernel(const __grid_
                 for (int q = warp - 4; q < share; q += kEpiWarps) {
                     const int column = cta * share + q, in_tile = column / each * half + s * 16 + column % each;
                     if (in_tile >= t.rows) continue;
-                    float v[2][4] = {};
+                    float v[kAcc][4] = {};
                     for (int c = 0; c < ctas; ++c)
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const float4 p = *reinterpret_cast<const float4*>(&sh.parts[((c * share + q) * 2 + i) * kLanes + lane * 4]);
+                        for (int i = 0; i < kAcc; ++i) {
+                            const float4 p = *reinterpret_cast<const float4*>(&sh.parts[((c * share + q) * kAcc + i) * kLanes + lane * 4]);
                             v[i][0] += p.x, v[i][1] += p.y, v[i][2] += p.z, v[i][3] += p.w;
                         }
                     const int64_t row = int64_t(t.row0) + in_tile;
                     if (kSwiGLU) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) v[0][j] = __fdividef(v[0][j], 1.f + __expf(-v[0][j])) * v[1][j];
+                        for (int j = 0; j < 4; ++j) v[0][j] = __fdividef(v[0][j], 1.f + __expf(-v[0][j])) * v[kAcc - 1][j];
                     } else if (args.row_scale != nullptr) {
                         const float f = args.row_scale[row];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) v[0][j] *= f, v[1][j] *= f;
+                        for (int i = 0; i < kAcc; ++i)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) v[i][j] *= f;
                     }
 #pragma unroll
-                    for (int i = 0; i < (kSwiGLU ? 1 : 2); ++i) {
-                        const int block = kSwiGLU ? t.nt : 2 * t.nt + i, n0 = block * 128 + lane * 4;
+                    for (int i = 0; i < (kSwiGLU ? 1 : kAcc); ++i) {
+                        const int block = kSwiGLU ? t.nt : kAcc * t.nt + i, n0 = block * 128 + lane * 4;
                         if (kQuantize) {
                             float m = 0.f;  // columns behind the last are zero
 #pragma unroll
@@ -440,10 +446,10 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_few_kernel(const __grid_
     }
 }
 
-template <bool kSwiGLU, bool kQuantize, int kTileRows>
+template <int kAcc, bool kSwiGLU, bool kQuantize, int kTileRows>
 cudaError_t launch_tile(const Maps& maps, const Args& args, int ctas, int64_t units, int sms, cudaStream_t stream) {
-    auto* fn = fp8_gemm_few_kernel<kSwiGLU, kQuantize, kTileRows>;
-    constexpr size_t kBytes = smem_bytes<kTileRows>();
+    auto* fn = fp8_gemm_few_kernel<kAcc, kSwiGLU, kQuantize, kTileRows>;
+    constexpr size_t kBytes = smem_bytes<kAcc, kTileRows>();
     static std::atomic<uint64_t> raised{0};
     const cudaError_t e = raise_shared_limit(fn, int(kBytes), raised);
     if (e != cudaSuccess) return e;
@@ -462,10 +468,10 @@ cudaError_t launch_tile(const Maps& maps, const Args& args, int ctas, int64_t un
     return cudaLaunchKernelEx(&config, fn, maps, args, ctas);
 }
 
-template <bool kSwiGLU, bool kQuantize>
+template <int kAcc, bool kSwiGLU, bool kQuantize>
 cudaError_t launch_mode(const Maps& maps, const Args& args, int tile, int ctas, int64_t units, int sms, cudaStream_t stream) {
-    if (tile <= 32) return launch_tile<kSwiGLU, kQuantize, 32>(maps, args, ctas, units, sms, stream);
-    return launch_tile<kSwiGLU, kQuantize, 64>(maps, args, ctas, units, sms, stream);
+    if (tile <= 32) return launch_tile<kAcc, kSwiGLU, kQuantize, 32>(maps, args, ctas, units, sms, stream);
+    return launch_tile<kAcc, kSwiGLU, kQuantize, 64>(maps, args, ctas, units, sms, stream);
 }
 
 }  // namespace
@@ -476,9 +482,11 @@ int few_clusters(int ctas, int sms) { return ctas <= 2 ? sms / ctas : ctas == 4 
 
 cudaError_t launch_few(const Maps& maps, const Args& args, int tile, int ctas, int64_t units, int sms, cudaStream_t stream) {
     if (args.experts > kMaxExperts || units < 1 || ctas < 1 || ctas > 8) return cudaErrorInvalidValue;
-    if (args.swiglu)
-        return args.q != nullptr ? launch_mode<true, true>(maps, args, tile, ctas, units, sms, stream) : launch_mode<true, false>(maps, args, tile, ctas, units, sms, stream);
-    return args.q != nullptr ? launch_mode<false, true>(maps, args, tile, ctas, units, sms, stream) : launch_mode<false, false>(maps, args, tile, ctas, units, sms, stream);
+    const bool q = args.q != nullptr;
+    if (args.swiglu) return q ? launch_mode<2, true, true>(maps, args, tile, ctas, units, sms, stream) : launch_mode<2, true, false>(maps, args, tile, ctas, units, sms, stream);
+    if (args.n_tiles == args.n_blocks)
+        return q ? launch_mode<1, false, true>(maps, args, tile, ctas, units, sms, stream) : launch_mode<1, false, false>(maps, args, tile, ctas, units, sms, stream);
+    return q ? launch_mode<2, false, true>(maps, args, tile, ctas, units, sms, stream) : launch_mode<2, false, false>(maps, args, tile, ctas, units, sms, stream);
 }
 
 }  // namespace fp8

@@ -29,7 +29,7 @@ struct Args {
     int64_t rows;
     int experts, n;                 // n: output columns (with SwiGLU half of the weight's rows)
     int k_blocks, n_blocks;         // of 128
-    int n_tiles;                    // of 256 output columns (128 with SwiGLU)
+    int n_tiles;                    // of 256 output columns; of 128 with SwiGLU, or (few rows) where that many are given
     int swiglu;
     uint32_t* status;               // 2 words: first error code, detail
     uint64_t timeout_ns;

@@ -352,25 +352,32 @@ void check_i64(const OptTensor& t, const at::Tensor& a, int64_t entries, const c
 // rows as N, 64, and rows as M: 32 rows an expert 157, 166, 172; 64 rows 199, 192, 174.  One matrix of 7168 x 4096: one row 14 over four
 // CTAs, 27 in one, 35; 128 rows 27, 21, 38.
 struct Fp8Choice {
-    int64_t tile, ctas, units;
+    int64_t tile, ctas, units, n_tiles;
 };
-Fp8Choice choose_fp8(int64_t rows, int64_t experts, int64_t most, int64_t n_tiles, int64_t k_blocks, int64_t sms, int64_t tile, int64_t ctas) {
+Fp8Choice choose_fp8(int64_t rows, int64_t experts, int64_t most, int64_t n_blocks, bool swiglu, int64_t k_blocks, int64_t sms, int64_t tile, int64_t ctas,
+                     int64_t columns) {
     const int64_t holders = std::min(experts, rows), average = std::max((rows + holders - 1) / holders, most > 0 && most <= 32 ? most : 1);
     const auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
     Fp8Choice c{};
+    constexpr double kHalfTile = 0.62;  // a block of a tile of 128 columns, of one of 256
     double best = -1;
     for (const int64_t t : {int64_t(32), int64_t(64), int64_t(128)}) {
         if (tile > 0 && t != tile) continue;
-        const int64_t tiles = up(average, t), units = holders * tiles * n_tiles;
-        for (int64_t s = 1; s <= (t == 128 ? 1 : 8); s *= 2) {
-            if (ctas > 0 && s != ctas && t != 128) continue;
-            const int64_t clusters = fp8::few_clusters(int(s), int(sms));
-            const double busy = double(std::min(units, clusters) * s) / double(sms);
-            const double block = t == 128 ? 0.62 + 0.07 * busy : t == 64 ? 0.61 + 0.25 * busy : tiles > 1 ? 0.45 : 0.43 + 0.27 * busy;
-            const double time = double(up(units, clusters)) * (double(up(k_blocks, s)) * block + (t == 128 ? 2.7 : 2.5 + 0.3 * double(s)));
-            if (best >= 0 && time >= best) continue;
-            best = time;
-            c = Fp8Choice{t, s, (rows / t + holders) * n_tiles};
+        for (int64_t wide = swiglu ? 1 : 2; wide >= 1; --wide) {  // blocks of 128 columns a tile: one is for calls that leave SMs idle
+            if ((wide == 1 && !swiglu && t == 128) || (columns > 0 && !swiglu && t < 128 && columns != wide * 128)) continue;
+            const bool half = wide == 1 && !swiglu;
+            const int64_t n_tiles = up(n_blocks, wide), tiles = up(average, t), units = holders * tiles * n_tiles;
+            for (int64_t s = 1; s <= (t == 128 ? 1 : 8); s *= 2) {
+                if (ctas > 0 && s != ctas && t != 128) continue;
+                const int64_t clusters = fp8::few_clusters(int(s), int(sms));
+                const double busy = double(std::min(units, clusters) * s) / double(sms);
+                double block = t == 128 ? 0.62 + 0.07 * busy : t == 64 ? 0.61 + 0.25 * busy : tiles > 1 ? 0.45 : 0.43 + 0.27 * busy;
+                if (half) block *= kHalfTile;
+                const double time = double(up(units, clusters)) * (double(up(k_blocks, s)) * block + (t == 128 ? 2.7 : 2.5 + 0.3 * double(s)));
+                if (best >= 0 && time >= best) continue;
+                best = time;
+                c = Fp8Choice{t, s, (rows / t + holders) * n_tiles, n_tiles};
+            }
         }
     }
     return c;
@@ -379,7 +386,7 @@ Fp8Choice choose_fp8(int64_t rows, int64_t experts, int64_t most, int64_t n_tile
 // (out) or (q, scales)
 std::vector<at::Tensor> grouped_gemm_fp8(const at::Tensor& a, const at::Tensor& a_scales, const at::Tensor& w, const at::Tensor& w_scales,
                                          const OptTensor& expert_offsets, const OptTensor& expert_counts, const OptTensor& row_scale, bool swiglu, bool quantize,
-                                         int64_t max_expert_rows, const at::Tensor& status, int64_t tile, int64_t ctas) {
+                                         int64_t max_expert_rows, const at::Tensor& status, int64_t tile, int64_t ctas, int64_t columns) {
     check_e4m3(a, 2, "a");
     check_e4m3(w, 3, "w");
     const int64_t rows = a.size(0), K = a.size(1), E = w.size(0), halves = swiglu ? 2 : 1;
@@ -408,6 +415,7 @@ std::vector<at::Tensor> grouped_gemm_fp8(const at::Tensor& a, const at::Tensor& 
     TORCH_CHECK(max_expert_rows >= 0, "max_expert_rows must not be negative");
     TORCH_CHECK((tile == 0 || tile == 32 || tile == 64 || tile == 128) && (ctas == 0 || ctas == 1 || ctas == 2 || ctas == 4 || ctas == 8),
                 "tile must be 0, 32, 64 or 128 and ctas 0, 1, 2, 4 or 8");
+    TORCH_CHECK(columns == 0 || columns == 128 || columns == 256, "columns must be 0, 128 or 256");
     check_status_tensor(status, a);
     c10::cuda::CUDAGuard guard(a.device());
     std::vector<at::Tensor> out;
@@ -435,12 +443,12 @@ std::vector<at::Tensor> grouped_gemm_fp8(const at::Tensor& a, const at::Tensor& 
     g.n = int(n);
     g.k_blocks = int(kb);
     g.n_blocks = int(nb);
-    g.n_tiles = int(swiglu ? nb : (nb + 1) / 2);
     g.swiglu = swiglu;
     g.status = reinterpret_cast<uint32_t*>(status.data_ptr<int>());
     g.timeout_ns = uint64_t(5e9);
     const int sms = sm_count();
-    const Fp8Choice c = choose_fp8(rows, E, max_expert_rows, g.n_tiles, g.k_blocks, sms, tile, ctas);
+    const Fp8Choice c = choose_fp8(rows, E, max_expert_rows, nb, swiglu, g.k_blocks, sms, tile, ctas, columns);
+    g.n_tiles = int(c.n_tiles);
     TORCH_CHECK(c.units < (int64_t(1) << 31), "too many output tiles for one call");
     fp8::Maps maps{};
     maps.weights = e4m3_map(w.data_ptr(), K, n, E * halves, swiglu && c.tile == 128 ? 64 : 128);
@@ -559,12 +567,12 @@ void bind_ops(pybind11::module_& m) {
     m.def("sort_tokens", &sort_tokens, py::arg("x"), py::arg("slots"), py::arg("slot_map"), py::arg("scales"), py::arg("zero_padding"));
     m.def("unsort_tokens", &unsort_tokens, py::arg("y"), py::arg("slots"), py::arg("slot_map"), py::arg("weights"), py::arg("bias"));
     m.def("unsort_tokens_grad", &unsort_tokens_grad, py::arg("grad_out"), py::arg("y"), py::arg("slots"), py::arg("slot_map"), py::arg("weights"));
-    m.def("fp8_gemm_choice", [](int64_t rows, int64_t experts, int64_t most, int64_t n_tiles, int64_t k_blocks, int64_t sms) {
-        const Fp8Choice c = choose_fp8(rows, experts, most, n_tiles, k_blocks, sms, 0, 0);
-        return std::make_pair(c.tile, c.ctas);
+    m.def("fp8_gemm_choice", [](int64_t rows, int64_t experts, int64_t most, int64_t n_blocks, bool swiglu, int64_t k_blocks, int64_t sms) {
+        const Fp8Choice c = choose_fp8(rows, experts, most, n_blocks, swiglu, k_blocks, sms, 0, 0, 0);
+        return std::make_tuple(c.tile, c.ctas, c.n_tiles);
     });
     m.def("grouped_gemm_fp8", &grouped_gemm_fp8, py::arg("a"), py::arg("a_scales"), py::arg("w"), py::arg("w_scales"), py::arg("expert_offsets"),
-          py::arg("expert_counts"), py::arg("row_scale"), py::arg("swiglu"), py::arg("quantize"), py::arg("max_expert_rows"), py::arg("status"), py::arg("tile") = 0, py::arg("ctas") = 0);
+          py::arg("expert_counts"), py::arg("row_scale"), py::arg("swiglu"), py::arg("quantize"), py::arg("max_expert_rows"), py::arg("status"), py::arg("tile") = 0, py::arg("ctas") = 0, py::arg("columns") = 0);
 }
 
 }  // namespace nep

@@ -58,7 +58,7 @@ def unsort_tokens(y: torch.Tensor, order: TokenOrder, weights: torch.Tensor | No
     """``out[t] = bias[t] + sum_k weights[t, k] * y[order.slots[t, k]]``, summed in FP32 in ascending ``k`` and rounded once.
 
     ``y`` bf16, fp16 or fp32 ``[C, H]`` (rows without a choice are not read), ``weights`` fp32 ``[T, K]`` (ones without; those of masked
-    choices are not read), ``bias`` ``[T, H]`` of ``y``'s type.  Differentiable in all three.
+    choices may be anything), ``bias`` ``[T, H]`` of ``y``'s type.  Differentiable in all three.
     """
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (y, weights, bias)):
         refuse_captured_gradients("unsort_tokens", "unsort_tokens_grad")

@@ -136,13 +136,14 @@ def test_rows_that_do_not_exist(alignment, tail, quantize):
 
 
 @pytest.mark.parametrize("counts", [[1], [16], [17, 0, 40], [129, 300, 0, 5], [33, 64, 65, 128, 256, 257]])
-@pytest.mark.parametrize("tile,ctas", [(32, 1), (32, 2), (32, 4), (32, 8), (64, 1), (64, 2), (64, 8), (128, 1)])
+@pytest.mark.parametrize("tile,ctas,columns", [(32, 1, 0), (32, 2, 256), (32, 4, 256), (32, 8, 256), (64, 1, 256), (64, 2, 256), (64, 8, 256), (128, 1, 0), (32, 1, 128), (32, 4, 128),
+                                               (64, 2, 128), (64, 8, 128)])
 @pytest.mark.parametrize("K,n,swiglu,quantize,scaled", [(128, 48, False, False, True), (2064, 400, False, True, False), (1024, 384, True, True, False), (400, 144, True, False, False)])
-def test_every_kernel(counts, tile, ctas, K, n, swiglu, quantize, scaled):
+def test_every_kernel(counts, tile, ctas, columns, K, n, swiglu, quantize, scaled):
     """Every tile and split of the K axis, also where a CTA's part of it is empty."""
     a, sa, w, sw, offsets, c, real = _problem(counts, K, 2 * n if swiglu else n, swiglu=swiglu, tail=2)
     scale = torch.rand(len(a), device="cuda") + 0.5 if scaled else None
-    got = gg._ext().grouped_gemm_fp8(a, sa, w, sw, offsets, None, scale, swiglu, quantize, 0, gg.status_tensor(a.device), tile, ctas)
+    got = gg._ext().grouped_gemm_fp8(a, sa, w, sw, offsets, None, scale, swiglu, quantize, 0, gg.status_tensor(a.device), tile, ctas, columns)
     gg.check_status()
     want, off = _reference(a, sa, w, sw, offsets, c, swiglu, scale)
     if quantize:
@@ -190,8 +191,10 @@ def test_a_row_does_not_depend_on_the_others():
 
 @pytest.mark.parametrize("rows,experts,most,k_blocks", [(1, 1, 1, 56), (64, 1, 0, 16), (512, 32, 32, 56), (512, 32, 0, 56), (4096, 32, 0, 16), (40000, 32, 0, 56), (7, 256, 0, 8), (3, 3, 900, 1)])
 def test_the_choice_covers_every_call(rows, experts, most, k_blocks):
-    tile, ctas = gg._ext().fp8_gemm_choice(rows, experts, most, 16, k_blocks, 148)
-    assert tile in (32, 64, 128) and ctas in (1, 2, 4, 8) and (tile < 128 or ctas == 1)
+    for swiglu in (False, True):
+        tile, ctas, n_tiles = gg._ext().fp8_gemm_choice(rows, experts, most, 16, swiglu, k_blocks, 148)
+        assert tile in (32, 64, 128) and ctas in (1, 2, 4, 8) and (tile < 128 or ctas == 1)
+        assert n_tiles == 16 if swiglu else n_tiles in (8, 16) and (tile < 128 or n_tiles == 8)
 
 
 def test_extreme_scales_and_values():

@@ -5,11 +5,16 @@ about 2^-4 / sqrt(3) = 0.036 at the coarse end of a binade.  The reference makes
 the layer's 32-bit sum may fall on the other side, an error of one step of one value in thousands.  2-norm of the difference below 0.02 of
 the result leaves room for the bf16 roundings (2^-8 each) and for those; a missing or doubled row shows as a multiple of it."""
 
+from datetime import timedelta
+
 import pytest
 import torch
+import torch.distributed as dist
 
+from nanoep_b200 import CudaBuffer, EPConfig
 from nanoep_b200.models.quantized_moe import QuantizedMoE
 from nanoep_b200.ops import grouped_gemm as gg
+from nanoep_b200.ops.fp8_gemm import grouped_gemm_fp8, quantize_rows
 from nanoep_b200.ops.rms_norm import rms_norm
 
 pytestmark = pytest.mark.gpu
@@ -85,6 +90,32 @@ def test_layer(tokens, hidden, inner, experts, topk, norm):
         _near(out, want)
         assert torch.equal(stream, h)
     gg.check_status()
+
+
+def test_between_dispatch_and_combine(monkeypatch):
+    """The 8-bit products on a dispatch's rows: aligned ranges, counts that leave padding rows out, gate weights in the product, and a combine behind them."""
+    monkeypatch.setenv("LOCAL_RANK", "0")
+    monkeypatch.setenv("LOCAL_WORLD_SIZE", "1")
+    layer = _layer(8, 512, 256, norm=False)
+    x, idx, gate = _batch(300, 512, 8, 4)
+    own = not dist.is_initialized()
+    if own:
+        dist.init_process_group("gloo", store=dist.HashStore(), rank=0, world_size=1, timeout=timedelta(seconds=60))
+    try:
+        with CudaBuffer(dist.group.WORLD, EPConfig(8, 4, 512, 300)) as buf:
+            got = buf.dispatch(x, topk_idx=idx, weights=gate, do_expand=True, alignment=128)
+            layout = got.handle.layout
+            ranges = dict(expert_counts=layout.expert_counts, max_expert_rows=layout.recv_count)
+            q, scales = grouped_gemm_fp8(*quantize_rows(got.x), layer.w13, layer.w13_scales, layout.expert_offsets, swiglu=True, quantize=True, **ranges)
+            y = grouped_gemm_fp8(q, scales, layer.w2, layer.w2_scales, layout.expert_offsets, row_scale=got.topk_weights, **ranges)
+            out = buf.combine(y, got.handle).x
+            torch.cuda.synchronize()
+            buf.check_status()
+            gg.check_status()
+    finally:
+        if own:
+            dist.destroy_process_group()
+    _near(out, _reference(layer, x, idx, gate, None)[0])
 
 
 def test_router_sees_the_normed_rows():

@@ -182,10 +182,10 @@ def test_gradients_of_some_inputs_and_once():
         out = unsort_tokens(leaves[0], order, leaves[1], bias=leaves[2])
         for i, grad in zip(wanted, torch.autograd.grad(out, [leaves[i] for i in wanted], g)):
             assert torch.equal(grad, (*full, g)[i])
-    x = torch.randn(9, 32, device="cuda", requires_grad=True)
-    for out in (sort_tokens(x, order).sum(), unsort_tokens(y.clone().requires_grad_() * 1, order).sum()):
+    x, leaf = torch.randn(9, 32, device="cuda", requires_grad=True), y.clone().requires_grad_()
+    for out, of in ((sort_tokens(x, order), x), (unsort_tokens(leaf, order), leaf)):
         with pytest.raises(RuntimeError, match="create_graph"):
-            out.backward(create_graph=True)
+            torch.autograd.grad(out.sum(), of, create_graph=True)
 
 
 def test_an_expert_id_out_of_range_is_masked_and_reported():
