@@ -6,14 +6,15 @@
 // needed per column: it comes from shared memory, four columns a load, cheap as long as there are few.
 //
 // A CTA computes 256 weight rows x N rows as two accumulators of 128 TMEM lanes: gate and up rows of the same 128 features with SwiGLU, so that
-// a lane holds both factors of its outputs, or two neighbouring blocks of output columns.  A cluster of S CTAs splits the K axis: S times the
+// a lane holds both factors of its outputs, or two neighbouring blocks of output columns; where tiles are so few that SMs stay idle, one
+// block (128 weight rows).  A cluster of S CTAs splits the K axis: S times the
 // SMs on one weight tile where there are few tiles, and an even share where their number is no multiple of the SMs.
 // The CTAs exchange their sums through distributed shared memory, 32 rows at a time; each finishes its share of the rows, adding
 // the parts in the order of K.  On the way the tile is turned: a warp finishes whole output rows.
 //
 // What bounds it: the weights' way from memory (32 experts of 7168 x 2048, up, us: 1 row each 150, 16 rows 154, 32 rows 159 = 5.9 TB/s, where a
 // copy runs at 6.5; rows as M 171, 172, 176), and for one matrix that of few SMs, 78 GB/s each, behind about 8 us of launch, setup and
-// exchange: 7168 x 4096 with one row 28.5 us in one CTA a tile, 18.5 in two, 14.4 in four.
+// exchange: 7168 x 4096 with one row 28.5 us in one CTA a tile, 18.5 in two, 14.1 in four, 12.4 in four on tiles of 128 weight rows.
 //
 // Tried: 16 columns of both accumulators per wait instead of 8: 64 rows each 193 -> 200 us; the state of the next barriers asked for under the
 // MMAs: within the spread; 128 rows as N: 312 us at 128 rows each (the columns' scales), rows as M 188.
