@@ -57,10 +57,10 @@ struct Shared {
     int4 tile[2];                                  // of the chunk's blocks: expert, first row, rows, weight tile
     float row_scales[2][kScaleBlocks][kTileRows];  // of the next blocks, by turns
     float weight_scales[2][kScaleBlocks][2];       // of the tile's two halves (of the gate and up rows)
-    float most[2][2][kTileRows];                   // largest of each row's 64 columns, by parity of the tile and epilogue group
+    float most[kExchangeTurns][2][kTileRows];      // largest of each row's 64 columns, by turn and epilogue group
     uint64_t full[kStages], done[kStages], tmem_empty[2];
     uint64_t scale_full[2], scale_empty[2];
-    uint64_t told[2][4];                           // by epilogue group and quarter: its rows' largest values are in `most`
+    uint64_t told[kExchangeTurns][2][4];           // by the same, and quarter: its rows' largest values are in `most`
     uint32_t tmem_base;
     int abort;
     int first_tile[kMaxExperts + 1];               // exclusive prefix of row tiles
@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
             mbar_init(&sh.scale_full[b], 1);
             mbar_init(&sh.scale_empty[b], kEpiWarps);
         }
-        for (int q = 0; q < 8; ++q) mbar_init(&sh.told[q >> 2][q & 3], 1);
+        for (int q = 0; q < kExchangeTurns * 8; ++q) mbar_init(&sh.told[q >> 3][q >> 2 & 1][q & 3], 1);
         sh.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -414,18 +414,17 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
 #pragma unroll
                 for (int j = 0; j < kCols; ++j) m = max_nan(m, fabsf(acc[j]));  // columns behind the last are zero
                 if (kSwiGLU) {
-                    // The other group's warp of the same rows has the block's other 64 columns.  What it told for a tile has been read before
-                    // this warp tells for the next one, so two places by turns are enough.
-                    const int turn = exchanges & 1;
-                    sh.most[turn][group][r] = m;
+                    // The other group's warp of the same rows has the block's other 64 columns.
+                    const ExchangeTurn turn = exchange_turn(exchanges);
+                    sh.most[turn.at][group][r] = m;
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&sh.told[group][quarter]);
-                    ok = __all_sync(0xffffffffu, wait_block(&sh.told[group ^ 1][quarter], uint32_t(turn), limit_ns, abort_flag));
+                    if (lane == 0) mbar_arrive(&sh.told[turn.at][group][quarter]);
+                    ok = __all_sync(0xffffffffu, wait_block(&sh.told[turn.at][group ^ 1][quarter], turn.parity, limit_ns, abort_flag));
                     if (!ok) {
                         if (lane == 0) fail(kPipeTimeout);
                         break;
                     }
-                    m = max_nan(m, sh.most[turn][group ^ 1][r]);
+                    m = max_nan(m, sh.most[turn.at][group ^ 1][r]);
                     ++exchanges;
                 }
                 m = max_nan(m, kTiny);

@@ -5,11 +5,24 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include "layout.hpp"
+
 namespace nep {
 namespace fp8 {
 
 constexpr int kMaxExperts = 1024;
 enum Fp8Status : uint32_t { kPipeTimeout = 101, kBadOffsets = 106 };
+
+// Two warps that hold one output block's columns swap their rows' largest values, tile after tile: each writes its own, arrives on its barrier and waits
+// for the other's arrival.  Nothing else holds the two together where K has one or two blocks: a warp may arrive for the next tile before the other one has
+// looked at its arrival for this tile, but it waits there for what the other tells for that next tile, behind the look.  So two turns are enough, with
+// a barrier each: one barrier for both could go through two phases between two looks, and the wait for the first would not end.
+constexpr int kExchangeTurns = 2;
+struct ExchangeTurn {
+    int at;           // place of the values, and of the barrier
+    uint32_t parity;  // of that barrier's phase
+};
+NEP_HD ExchangeTurn exchange_turn(int exchange) { return ExchangeTurn{exchange % kExchangeTurns, uint32_t(exchange / kExchangeTurns) & 1u}; }
 
 // Tensor maps: rows in boxes of 128, 64, 32 and 16 (by 128 columns), weights [experts (* 2)][n][k].
 struct Maps {

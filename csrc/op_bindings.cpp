@@ -568,6 +568,10 @@ void bind_ops(pybind11::module_& m) {
     m.def("sort_tokens", &sort_tokens, py::arg("x"), py::arg("slots"), py::arg("slot_map"), py::arg("scales"), py::arg("zero_padding"));
     m.def("unsort_tokens", &unsort_tokens, py::arg("y"), py::arg("slots"), py::arg("slot_map"), py::arg("weights"), py::arg("bias"));
     m.def("unsort_tokens_grad", &unsort_tokens_grad, py::arg("grad_out"), py::arg("y"), py::arg("slots"), py::arg("slot_map"), py::arg("weights"));
+    m.def("exchange_turn", [](int exchange) {
+        const auto turn = fp8::exchange_turn(exchange);
+        return std::make_pair(turn.at, turn.parity);
+    });
     m.def("fp8_gemm_choice", [](int64_t rows, int64_t experts, int64_t most, int64_t n_blocks, bool swiglu, int64_t k_blocks, int64_t sms) {
         const Fp8Choice c = choose_fp8(rows, experts, most, n_blocks, swiglu, k_blocks, sms, 0, 0, 0);
         return std::make_tuple(c.tile, c.ctas, c.n_tiles);

@@ -152,6 +152,24 @@ def test_every_kernel(counts, tile, ctas, columns, K, n, swiglu, quantize, scale
         _check(got[0], want, off, real)
 
 
+@pytest.mark.parametrize("K", [112, 256, 384, 1024, 1136])
+@pytest.mark.parametrize("swiglu,quantize,scaled", [(False, False, False), (False, False, True), (False, True, False), (True, False, False), (True, True, False)])
+def test_several_tiles_a_block(K, swiglu, quantize, scaled):
+    """Rows as M on more than twice as many tiles as the GPU holds, full ones beside those of a few rows, over one to nine blocks of K."""
+    n, counts = 1040, [e * 37 % 300 + 1 for e in range(40)]
+    tiles = sum(-(-c // 128) for c in counts) * (-(-n // 128) if swiglu else -(-n // 256))
+    assert tiles > 2 * torch.cuda.get_device_properties(0).multi_processor_count and any(c % 128 and c % 128 <= 32 for c in counts)
+    a, sa, w, sw, offsets, c, real = _problem(counts, K, 2 * n if swiglu else n, swiglu=swiglu, tail=2)
+    scale = torch.rand(len(a), device="cuda") + 0.5 if scaled else None
+    got = gg._ext().grouped_gemm_fp8(a, sa, w, sw, offsets, None, scale, swiglu, quantize, 0, gg.status_tensor(a.device), 128, 1, 0)
+    gg.check_status()
+    want, off = _reference(a, sa, w, sw, offsets, c, swiglu, scale)
+    if quantize:
+        _check_quantized(*got, want, off, real)
+    else:
+        _check(got[0], want, off, real)
+
+
 @pytest.mark.parametrize("rows", [1, 3, 64, 129])
 def test_one_matrix(rows):
     a, sa, w, sw, offsets, n, real = _problem([rows], 768, 384)
