@@ -4,7 +4,8 @@
     y[t] = sum_k w[t,k] * W2[e_k] @ q( silu(W1g[e_k] @ n[t]) * (W1u[e_k] @ n[t]) )
 
 The layer of ``moe_layer.ExpertParallelMoE`` without a group: no peer window and no wait of the host, so a step can be captured in a
-CUDA graph.  Rows travel between its kernels in 8 bits with a scale for each 128 columns; down-projected rows in bf16.
+CUDA graph.  Rows travel between its kernels in 8 bits with a scale for each 128 columns; down-projected rows in bf16.  It serves: the experts
+have no gradient, so with autograd on (outside of ``torch.no_grad()``) nothing that comes into the layer may require one.
 """
 
 from __future__ import annotations
@@ -12,6 +13,7 @@ from __future__ import annotations
 import torch
 
 from ..ops.fp8_gemm import grouped_gemm_fp8, quantize_rows, quantize_weights
+from ..ops.grouped_gemm import refuse_gradients
 from ..ops.rms_norm import rms_norm
 from ..ops.token_order import plan_tokens, sort_tokens, unsort_tokens
 
@@ -41,6 +43,7 @@ class QuantizedMoE:
                 residual: torch.Tensor | None = None, router=None, bias: torch.Tensor | None = None):
         """``x`` ``[T, H]``; ``topk_idx`` int64 ``[T, K]`` (-1 = masked) and ``topk_weights`` fp32 ``[T, K]``, or ``router``, which gives both from the normed rows.
         Returns ``out`` bf16 ``[T, H]`` (plus ``bias`` ``[T, H]``, a shared expert's output), or ``(out, x + residual)`` where a ``residual`` is given."""
+        refuse_gradients("QuantizedMoE", x, topk_weights, residual, bias, self.norm_weight, self.w13, self.w13_scales, self.w2, self.w2_scales)
         stream = None
         if self.norm_weight is not None:
             normed = rms_norm(x, self.norm_weight, residual=residual, eps=self.eps, quantize=True, keep=router is not None)
@@ -52,6 +55,7 @@ class QuantizedMoE:
             q, scales = quantize_rows(x)
         if router is not None:
             topk_idx, topk_weights = router(rows)
+            refuse_gradients("QuantizedMoE", topk_weights)
         order = plan_tokens(topk_idx, self.num_experts)
         q, scales = sort_tokens(q, order, scales=scales)
         q, scales = grouped_gemm_fp8(q, scales, self.w13, self.w13_scales, order.expert_offsets, swiglu=True, quantize=True)

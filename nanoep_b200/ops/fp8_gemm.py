@@ -1,7 +1,7 @@
 """Grouped GEMM of e4m3 rows and e4m3 expert weights with a scale for each block of 128 (csrc/fp8_gemm_sm100.cu).
 
 Rows carry one fp32 scale for each 128 columns, weights one for each 128 x 128 block, of any positive value.  Half the bytes of the
-bf16 experts in decode, twice the tensor rate in prefill.  A serving operator: it has no gradient.
+bf16 experts in decode, twice the tensor rate in prefill.  Serving operators: they have no gradient, and with autograd on they refuse tensors that require one.
 """
 
 from __future__ import annotations
@@ -9,7 +9,7 @@ from __future__ import annotations
 import torch
 
 from ..utils.build import load_extension as _ext
-from .grouped_gemm import operator_status
+from .grouped_gemm import operator_status, refuse_gradients
 
 BLOCK = 128
 LARGEST = 448.0  # of e4m3
@@ -19,12 +19,15 @@ TINY = 1e-30     # smallest value that a block is scaled by
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """bf16, fp16 or fp32 ``[rows, K]`` -> ``(q, scales)``: e4m3 ``[rows, K]`` and fp32 ``[rows, ceil(K / 128)]`` with ``q * scales = x``,
     ``scales = max(max |x|, 1e-30) / 448`` of each 128 columns."""
+    refuse_gradients("quantize_rows", x)
     return _ext().quantize_rows(x)
 
 
+@torch.no_grad()
 def quantize_weights(w: torch.Tensor, *, swiglu: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
     """``[E, N, K]`` or ``[N, K]`` weights -> e4m3 weights and a fp32 scale for each 128 x 128 block.  With ``swiglu`` (``N = 2 * I``: gate rows,
-    then up rows) the halves have blocks of their own.  For loading a model: plain torch operations, one expert at a time."""
+    then up rows) the halves have blocks of their own.  For loading a model: plain torch operations, one expert at a time;
+    what it returns requires no gradient."""
     if w.dim() == 2:
         q, scales = quantize_weights(w[None], swiglu=swiglu)
         return q[0], scales[0]
@@ -61,6 +64,7 @@ def grouped_gemm_fp8(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w
     ``max_expert_rows`` (0 = unknown): no expert holds more rows; the choice of the tile goes by it, the result only in
     its rounding.
     """
+    refuse_gradients("grouped_gemm_fp8", a, a_scales, w, w_scales, row_scale)
     if w.dim() == 2:
         w, w_scales = w[None], w_scales[None]
     out = _ext().grouped_gemm_fp8(a, a_scales, w, w_scales, expert_offsets, expert_counts, row_scale, bool(swiglu), bool(quantize),

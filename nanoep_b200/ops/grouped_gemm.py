@@ -49,6 +49,12 @@ def refuse_captured_gradients(name: str, explicit: str):
         raise RuntimeError(f"{name} is not differentiated inside a CUDA graph capture: call {explicit} there")
 
 
+def refuse_gradients(name: str, *tensors):
+    """For operators without a gradient: a result that is cut off from autograd's graph looks like one that depends on less than it does."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError(f"{name} has no gradient and got a tensor that requires one: call it under torch.no_grad(), or with detached tensors")
+
+
 def check_status(device=None):
     """Raise if a kernel of these operators on ``device`` gave up on a bounded wait or met invalid indices (synchronises)."""
     st = status_tensor(device if device is not None else torch.cuda.current_device())
@@ -71,6 +77,7 @@ def grouped_gemm(a, w, expert_offsets, *, swiglu: bool = False, out=None, tile_r
     ``row_scale`` (fp32 ``[rows]``, plain mode) multiplies each output row in FP32 before the bf16 round.
     ``expert_counts`` (int64 ``[E]``): only so many rows of each expert's range exist; the other rows are neither read as
     far as the result goes nor defined in the output.  ``max_expert_rows`` (0 = unknown): no expert holds more rows.
+    It has no gradient: autograd sees its result as a constant.
     ``stages=3`` runs the single-CTA kernel with a pipeline that leaves a third of an SM's shared memory to another kernel,
     ``pair=True`` the CTA-pair kernel (two SMs share every weight tile); both compute every row of every range, and they are
     what runs with ``tile_ready`` (row blocks gated by counters).

@@ -45,7 +45,7 @@ def sort_tokens(x: torch.Tensor, order: TokenOrder, *, scales: torch.Tensor | No
     ``scales`` (fp32 ``[T, blocks]``, of 8-bit rows) travels along, and ``(rows, row_scales)`` is returned.  With ``zero_padding`` every row
     without a choice is zero, otherwise it is not written.  Differentiable in ``x`` (without ``scales``).
     """
-    if torch.is_grad_enabled() and x.requires_grad:
+    if torch.is_grad_enabled() and (x.requires_grad or (scales is not None and scales.requires_grad)):
         if scales is not None:
             raise ValueError("rows that travel with scales have no gradient")
         refuse_captured_gradients("sort_tokens", "sort_tokens_grad")

@@ -127,6 +127,22 @@ def test_router_sees_the_normed_rows():
     assert torch.equal(out, layer(x, idx, gate))
 
 
+def test_parameters_are_served_without_autograd():
+    """With autograd on, a router with parameters is refused like any input that needs a gradient; without, the layer gives what it gives for plain tensors."""
+    layer = _layer(8, 512, 256)
+    x, idx, gate = _batch(40, 512, 8, 2, masked=False)
+    want = layer(x, idx, gate)
+    scale = torch.nn.Parameter(torch.ones((), device="cuda"))
+    with pytest.raises(ValueError, match="no gradient"):
+        layer(x, router=lambda rows: (idx, gate * scale))
+    layer.norm_weight = torch.nn.Parameter(layer.norm_weight)
+    with pytest.raises(ValueError, match="no gradient"):
+        layer(x, idx, gate)
+    for off in (torch.no_grad(), torch.inference_mode()):
+        with off:
+            assert torch.equal(layer(x, router=lambda rows: (idx, gate * scale)), want)
+
+
 def test_every_choice_masked():
     layer = _layer(4, 256, 128)
     x = torch.randn(5, 256, device="cuda").to(torch.bfloat16)

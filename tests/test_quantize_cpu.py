@@ -3,9 +3,10 @@
 import pytest
 import torch
 
+from nanoep_b200.models.quantized_moe import QuantizedMoE
 from nanoep_b200.ops.fp8_gemm import grouped_gemm_fp8, quantize_rows, quantize_weights
 from nanoep_b200.ops.rms_norm import rms_norm
-from nanoep_b200.ops.token_order import plan_tokens
+from nanoep_b200.ops.token_order import TokenOrder, plan_tokens, sort_tokens
 
 
 @pytest.mark.parametrize("shape,swiglu", [((2, 256, 128), False), ((1, 16, 16), False), ((3, 272, 144), False), ((2, 2 * 144, 272), True), ((130, 260), False)])
@@ -41,3 +42,56 @@ def test_refusals():
     q, s = quantize_weights(torch.ones(128, 128))
     with pytest.raises(ValueError, match="CUDA"):
         grouped_gemm_fp8(q, s, q, s)
+
+
+def _needs(t):
+    return t.detach().clone().requires_grad_()
+
+
+def test_operators_without_a_gradient_refuse_tensors_that_need_one():
+    """Otherwise the result is a constant to autograd, and what is made of it a function of less than it is."""
+    x = torch.ones(4, 128)
+    (q, s), one = quantize_weights(torch.ones(128, 128)), torch.ones(4, 1)
+    rows = torch.ones(4, 128).to(torch.float8_e4m3fn)
+    for bad in (
+        lambda: quantize_rows(_needs(x)),
+        lambda: grouped_gemm_fp8(rows, _needs(one), q, s),
+        lambda: grouped_gemm_fp8(rows, one, q, _needs(s)),
+        lambda: grouped_gemm_fp8(rows, one, q, s, row_scale=_needs(one[:, 0])),
+    ):
+        with pytest.raises(ValueError, match="no gradient"):
+            bad()
+        with torch.no_grad(), pytest.raises((RuntimeError, ValueError), match="CUDA"):  # the next check
+            bad()
+    order = TokenOrder(*(torch.zeros(1, dtype=torch.int32) for _ in range(4)))
+    with pytest.raises(ValueError, match="no gradient"):
+        sort_tokens(rows, order, scales=_needs(one))
+
+
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("which", ["x", "residual", "norm_weight", "topk_weights", "bias", "router"])
+def test_the_layer_refuses_inputs_that_need_a_gradient(norm, which):
+    if not norm and which in ("residual", "norm_weight"):
+        pytest.skip("the norm's")
+    weight = torch.ones(128) if norm else None
+    layer = QuantizedMoE.quantize(torch.ones(2, 64, 128), torch.ones(2, 128, 32), norm_weight=_needs(weight) if which == "norm_weight" else weight)
+    given = dict(x=torch.ones(4, 128), topk_idx=torch.zeros(4, 1, dtype=torch.int64), topk_weights=torch.ones(4, 1))
+    if which in ("residual", "bias"):
+        given[which] = torch.ones(4, 128)
+    if which in given:
+        given[which] = _needs(given[which])
+    if which == "router":
+        del given["topk_idx"], given["topk_weights"]
+        given.update(x=_needs(given["x"]), router=lambda rows: pytest.fail("nothing runs before the refusal"))
+    with pytest.raises(ValueError, match="QuantizedMoE has no gradient"):
+        layer(**given)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):  # the next check: the operators'
+        layer(**given)
+
+
+def test_weights_in_8_bits_need_no_gradient():
+    """Of a model's parameters: the layer takes what comes back."""
+    q, s = quantize_weights(_needs(torch.randn(2, 160, 144)))
+    assert not q.requires_grad and not s.requires_grad
+    layer = QuantizedMoE.quantize(torch.nn.Parameter(torch.ones(2, 64, 128)), torch.nn.Parameter(torch.ones(2, 128, 32)))
+    assert not any(t.requires_grad for t in (layer.w13, layer.w13_scales, layer.w2, layer.w2_scales))
