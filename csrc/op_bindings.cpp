@@ -357,7 +357,10 @@ struct Fp8Choice {
 };
 Fp8Choice choose_fp8(int64_t rows, int64_t experts, int64_t most, int64_t n_blocks, bool swiglu, int64_t k_blocks, int64_t sms, int64_t tile, int64_t ctas,
                      int64_t columns) {
-    const int64_t holders = std::min(experts, rows), average = std::max((rows + holders - 1) / holders, most > 0 && most <= 32 ? most : 1);
+    // Rows of an expert: the average of the ranges, which may be padded (to 128 behind a dispatch), and at most what the caller says.  An expert of up
+    // to 32 rows is one tile of any kind, so the largest of such a call counts rather than the average.
+    const int64_t holders = std::min(experts, rows), spread = (rows + holders - 1) / holders;
+    const int64_t average = most == 0 ? spread : most <= 32 ? most : std::min(spread, most);
     const auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
     Fp8Choice c{};
     constexpr double kHalfTile = 0.62;  // a block of a tile of 128 columns, of one of 256

@@ -7,6 +7,7 @@ from nanoep_b200.models.quantized_moe import QuantizedMoE
 from nanoep_b200.ops.fp8_gemm import grouped_gemm_fp8, quantize_rows, quantize_weights
 from nanoep_b200.ops.rms_norm import rms_norm
 from nanoep_b200.ops.token_order import TokenOrder, plan_tokens, sort_tokens
+from nanoep_b200.utils.build import load_extension
 
 
 @pytest.mark.parametrize("shape,swiglu", [((2, 256, 128), False), ((1, 16, 16), False), ((3, 272, 144), False), ((2, 2 * 144, 272), True), ((130, 260), False)])
@@ -95,3 +96,23 @@ def test_weights_in_8_bits_need_no_gradient():
     assert not q.requires_grad and not s.requires_grad
     layer = QuantizedMoE.quantize(torch.nn.Parameter(torch.ones(2, 64, 128)), torch.nn.Parameter(torch.ones(2, 128, 32)))
     assert not any(t.requires_grad for t in (layer.w13, layer.w13_scales, layer.w2, layer.w2_scales))
+
+
+@pytest.mark.parametrize("most", [1, 8, 16, 31, 33, 48, 64, 100])
+@pytest.mark.parametrize("experts", [1, 4, 32, 256])
+@pytest.mark.parametrize("swiglu", [False, True])
+def test_a_hint_goes_for_padded_ranges(most, experts, swiglu):
+    """Ranges of 128 rows in which no expert has more than ``most``: the kernel is that of ranges without padding."""
+    def choice(rows, hint):
+        return load_extension().fp8_gemm_choice(rows, experts, hint, 16, swiglu, 56, 148)
+
+    assert choice(experts * 128, most) == choice(experts * most, most)
+    assert choice(experts * 128, 128) == choice(experts * 128, 0) == choice(experts * 128, 5000)
+
+
+def test_few_rows_in_padded_ranges_run_on_tiles_of_few_rows():
+    choice = load_extension().fp8_gemm_choice
+    assert choice(4096, 32, 0, 16, True, 56, 148)[0] == 128
+    assert choice(4096, 32, 8, 16, True, 56, 148)[0] == choice(4096, 32, 32, 16, True, 56, 148)[0] == 32
+    for swiglu in (False, True):
+        assert choice(128, 1, 1, 16, swiglu, 56, 148) == choice(1, 1, 1, 16, swiglu, 56, 148)
