@@ -7,6 +7,7 @@
 #include "rms_norm.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 #include "row_prim.cuh"
 
@@ -17,6 +18,12 @@ namespace {
 using namespace rows;
 
 constexpr int kNormThreads = 512;
+
+// Products of two bf16 values have 16 bits.
+template <typename T, typename W>
+using ProductBlock = std::conditional_t<std::is_same<T, __nv_bfloat16>::value && std::is_same<W, __nv_bfloat16>::value, NarrowBlock, WideBlock>;
+template <typename T>
+using ValueBlock = std::conditional_t<std::is_same<T, float>::value, WideBlock, NarrowBlock>;
 
 // Sum over the block, the same value in every thread; `scratch` holds 32 floats and is free again after the next block barrier.
 __device__ __forceinline__ float block_sum(float v, float* scratch) {
@@ -95,11 +102,8 @@ __global__ void __launch_bounds__(kNormThreads, sizeof(T) + sizeof(W) == 4 && kU
             if (a.q != nullptr) {
                 m = max_nan(group_max<16>(m), kTiny);
                 if (u < units) {
-                    const Quotient of(m);
-                    uint2 q;
-                    q.x = pack_e4m3(of(f[0]), of(f[1]), of(f[2]), of(f[3]));
-                    q.y = pack_e4m3(of(f[4]), of(f[5]), of(f[6]), of(f[7]));
-                    *reinterpret_cast<uint2*>(a.q + row * a.hidden + u * 8) = q;
+                    const ProductBlock<T, W> block(m);
+                    *reinterpret_cast<uint2*>(a.q + row * a.hidden + u * 8) = make_uint2(block.pack(f), block.pack(f + 4));
                     if ((u & 15) == 0) a.scales[row * blocks + u / 16] = __fdiv_rn(m * rstd, kLargest);
                 }
             }
@@ -141,13 +145,14 @@ __global__ void __launch_bounds__(512) norm_any_kernel(const NormArgs a) {
             m = max_nan(m, fabsf(f[j]));
         }
         m = max_nan(group_max<32>(m), kTiny);
-        const Quotient of(m);
+        const ProductBlock<T, W> block(m);
+        const uint32_t q = a.q != nullptr ? block.pack(f) : 0u;
         if (a.q != nullptr && lane == 0) a.scales[row * blocks + b] = __fdiv_rn(m * rstd, kLargest);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int c = b * kBlock + j * 32 + lane;
             if (c >= a.hidden) continue;
-            if (a.q != nullptr) a.q[at + c] = __nv_cvt_float_to_fp8(of(f[j]), __NV_SATFINITE, __NV_E4M3);
+            if (a.q != nullptr) a.q[at + c] = uint8_t(q >> (8 * j));
             if (a.y != nullptr) static_cast<T*>(a.y)[at + c] = from_float<T>(f[j] * rstd);
         }
     }
@@ -291,10 +296,8 @@ __global__ void __launch_bounds__(256) quantize_kernel(const QuantizeArgs a) {
         m = max_nan(group_max<16>(m), kTiny);
         if (!inside) continue;
         if (part == 0) a.scales[b] = __fdiv_rn(m, kLargest);
-        const Quotient of(m);
-        uint2 q;
-        q.x = pack_e4m3(of(f[0]), of(f[1]), of(f[2]), of(f[3]));
-        q.y = pack_e4m3(of(f[4]), of(f[5]), of(f[6]), of(f[7]));
+        const ValueBlock<T> block_of(m);
+        const uint2 q = make_uint2(block_of.pack(f), block_of.pack(f + 4));
         if (a.aligned) {
             *reinterpret_cast<uint2*>(a.q + at) = q;
         } else {

@@ -104,6 +104,57 @@ def test_quantize_rows(rows, columns, dtype):
     _check_quantized(q, scales, x.double(), torch.ones(rows, 1, device="cuda", dtype=torch.float64), exact=dtype != torch.float32)
 
 
+def _nearest_e4m3(q):
+    """64-bit quotients of at most 448 to e4m3, rounded once (a conversion by torch goes through 32 bits, and rounds twice)."""
+    step = torch.exp2(torch.frexp(q.abs().clamp_min(2.0**-6)).exponent.double() - 4)
+    return torch.round(q / step) * step
+
+
+def _next_to_ties(v, m):
+    """Which quotients v * 448 / m are ties between two e4m3 values, or within 2^-21 of one."""
+    q = v.double() * 448 / m.double()
+    t = q / torch.exp2(torch.frexp(q.clamp_min(2.0**-6)).exponent.double() - 4)
+    return (t - t.floor() - 0.5).abs() < 2.0**-21 * t
+
+
+def test_ties_of_fp16_products():
+    """Products of 22 bits whose quotient is a tie or lies next to one: in 64 bits a quotient differs from a tie by 2^-31 at least."""
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    a, b, c, d = torch.randint(1024, 2048, (4, 1 << 25), generator=gen, device="cuda")
+    a, b, c, d = (torch.cat([torch.tensor(first, device="cuda"), t]) for first, t in zip(([1327, 1197], [1721, 2011], [1483, 441 * 4], [1597, 2011]), (a, b, c, d)))
+    # the second pair of the list: its quotient is 76, between 72 and 80, with the larger value four times as large
+    c = c * torch.where(torch.arange(len(c), device="cuda") % 2 == 1, 4, 1)
+    v, m = a * b, c * d
+    at = ((v <= m) & _next_to_ties(v, m)).nonzero().flatten()[:120]
+    assert len(at) == 120 and at[:2].tolist() == [0, 1]
+    for extra in (0, 1):  # the second width takes the kernel of any width
+        x, weight = torch.zeros(2, 128 * 120 + extra, device="cuda"), torch.ones(128 * 120 + extra, device="cuda")
+        first = torch.arange(120, device="cuda") * 128
+        x[0, first], x[0, first + 1], weight[first], weight[first + 1] = a[at].float(), c[at].float(), b[at].float(), d[at].float()
+        x[1] = -x[0]
+        got = rms_norm(x.half(), weight.half(), quantize=True)
+        want = _nearest_e4m3(v[at].double() * 448 / m[at].double())
+        assert torch.equal(got.q[0, first].double(), want) and torch.equal(got.q[1, first].double(), -want)
+        assert bool((got.q[0, first + 1].double() == 448).all())
+
+
+def test_ties_of_32_bit_values():
+    """24-bit values on both sides of every tie, and on it."""
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    blocks = 4096
+    m = torch.randint(1 << 23, 1 << 24, (blocks,), generator=gen, device="cuda").double()
+    m[::2] = torch.randint(1 << 17, 1 << 18, (blocks // 2,), generator=gen, device="cuda") * 56  # ties of these are exact: 448 = 8 * 56
+    ties = torch.tensor([t * 2.0**e for e in range(-4, 4) for t in range(17, 33, 2)] + [t * 2.0**-10 for t in (1, 3, 5, 7, 9, 11, 13, 15)], device="cuda", dtype=torch.float64)
+    on = (ties * m[:, None] / 448).float()
+    x = torch.zeros(blocks, 256, device="cuda")
+    x[:, :72], x[:, 128:200] = on, torch.nextafter(on, torch.zeros_like(on))
+    x[:, 72], x[:, 73:127], x[:, 200] = m.float(), torch.nextafter(on, torch.full_like(on, 1e30))[:, :54], m.float()
+    x *= torch.where(torch.rand(blocks, 256, generator=gen, device="cuda") < 0.5, -1, 1)
+    for scale in (1.0, 2.0**100, 2.0**-120):
+        q, _ = quantize_rows(x * scale)
+        assert torch.equal(q.double(), _nearest_e4m3(x.double() * 448 / m[:, None]))
+
+
 def _gradients(h, weight, rstd, gy, gh):
     """The formula's gradients in 64 bits, and the size of what is added up in each."""
     xhat, gw = h.double() * rstd, gy.double() * weight.double()
