@@ -423,10 +423,9 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_few_kernel(const __grid_
 #pragma unroll
                             for (int j = 0; j < 4; ++j) m = max_nan(m, fabsf(v[i][j]));
                             m = max_nan(group_max<32>(m), kTiny);
-                            const float per = __fdiv_rn(kLargest, m);  // sums do not lie on the border of two e4m3 values: a product will do
                             if (lane == 0 && block < args.n_blocks) args.scales[row * args.n_blocks + block] = __fdiv_rn(m, kLargest);
                             if (n0 < args.n)
-                                *reinterpret_cast<uint32_t*>(args.q + row * args.n + n0) = pack_e4m3(v[i][0] * per, v[i][1] * per, v[i][2] * per, v[i][3] * per);
+                                *reinterpret_cast<uint32_t*>(args.q + row * args.n + n0) = WideBlock(m).pack(v[i]);
                         } else if (n0 < args.n) {
                             *reinterpret_cast<uint2*>(args.out + row * args.n + n0) = make_uint2(pack_bf16(v[i][0], v[i][1]), pack_bf16(v[i][2], v[i][3]));
                         }

@@ -428,17 +428,19 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
                     ++exchanges;
                 }
                 m = max_nan(m, kTiny);
-                const float per = __fdiv_rn(kLargest, m);  // sums do not lie on the border of two e4m3 values: a product will do
+                const WideBlock scaled(m);
+                uint32_t unsure = 0;
                 if (real && (kSwiGLU ? group == 0 : inside)) args.scales[row * args.n_blocks + wb] = __fdiv_rn(m, kLargest);
 #pragma unroll
                 for (int j = 0; j < kCols; j += 16) {
                     uint32_t q[4];
 #pragma unroll
-                    for (int h = 0; h < 4; ++h) {
-                        const float* f = acc + j + 4 * h;
-                        q[h] = pack_e4m3(f[0] * per, f[1] * per, f[2] * per, f[3] * per);
-                    }
+                    for (int h = 0; h < 4; ++h) q[h] = scaled.guess(acc + j + 4 * h, unsure);
                     *reinterpret_cast<uint4*>(piece + j) = make_uint4(q[0], q[1], q[2], q[3]);
+                }
+                if (unsure != 0) {  // quotients next to a tie (this and the second product a value: 4096 tokens, 32 experts, up 1336 -> 1346 us)
+#pragma unroll
+                    for (int j = 0; j < kCols; j += 4) *reinterpret_cast<uint32_t*>(piece + j) = scaled.exact(acc + j);
                 }
                 if (real && n0 < args.n) send_piece(args.q + row * args.n + n0, piece, min(kCols, args.n - n0));
             } else {

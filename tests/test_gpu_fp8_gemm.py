@@ -170,6 +170,28 @@ def test_several_tiles_a_block(K, swiglu, quantize, scaled):
         _check(got[0], want, off, real)
 
 
+@pytest.mark.parametrize("tile", [32, 64, 128])
+def test_exact_sums_round_as_rows_do(tile):
+    """Sums of digits, exact in 32 bits: the e4m3 result is that of the quotient, ties to even, and what quantize_rows gives for the same values."""
+    gen = torch.Generator(device="cuda").manual_seed(tile)
+    rows, blocks = 300, 4
+    m = 28 * torch.randint(1, 2341, (rows, 1), generator=gen, device="cuda")  # 448 = 16 * 28: T * m / 28 is a whole number whose quotient is T * 16
+    tie = torch.randint(8, 14, (rows, 128), generator=gen, device="cuda") * 2 + 1
+    v = torch.where(torch.rand(rows, 128, generator=gen, device="cuda") < 0.5, tie * m // 28, torch.randint(0, 1 << 16, (rows, 128), generator=gen, device="cuda") % (m + 1))
+    v[:, 5:6] = m
+    digits = torch.cat([v >> 4 * b & 15 for b in range(blocks)], 1).float().to(E4M3)
+    a_scales = torch.tensor([16.0**b for b in range(blocks)], device="cuda").repeat(rows, 1)
+    w = torch.eye(128, device="cuda").repeat(1, blocks)[None].to(E4M3)
+    offsets = torch.tensor([0, rows], device="cuda")
+    q, scales = gg._ext().grouped_gemm_fp8(digits, a_scales, w, torch.ones(1, 1, blocks, device="cuda"), offsets, None, None, False, True, 0, gg.status_tensor(w.device), tile, 1, 0)
+    gg.check_status()
+    want = v.double() * 448 / m
+    step = torch.exp2(torch.frexp(want.clamp_min(2.0**-6)).exponent.double() - 4)
+    assert torch.equal(q.double(), torch.round(want / step) * step)
+    again = quantize_rows(v.float())
+    assert torch.equal(q.view(torch.uint8), again[0].view(torch.uint8)) and torch.equal(scales, again[1])
+
+
 @pytest.mark.parametrize("rows", [1, 3, 64, 129])
 def test_one_matrix(rows):
     a, sa, w, sw, offsets, n, real = _problem([rows], 768, 384)
