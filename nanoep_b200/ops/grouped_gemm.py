@@ -56,11 +56,13 @@ def refuse_gradients(name: str, *tensors):
 
 
 def check_status(device=None):
-    """Raise if a kernel of these operators on ``device`` gave up on a bounded wait or met invalid indices (synchronises)."""
+    """Raise if a kernel of these operators on ``device`` gave up on a bounded wait or met invalid indices.  Waits for the device, all its streams."""
     st = status_tensor(device if device is not None else torch.cuda.current_device())
+    torch.cuda.synchronize(st.device)
     code, cta = (int(v) for v in st[:2].tolist())
     if code != 0:
         st.zero_()
+        torch.cuda.synchronize(st.device)  # what another stream reports from here on stays
         reasons = {101: "an operand pipeline wait timed out", 102: "the wait for a row block's ready counter timed out",
                    103: "expert_offsets are not multiples of 128 from 0 to the row count", 104: "handle metadata names an impossible rank, token or row",
                    105: "an expert id lies outside [-1, num_experts)", 106: "expert_offsets fall, do not start at 0 or end behind the rows"}

@@ -197,6 +197,19 @@ def test_an_expert_id_out_of_range_is_masked_and_reported():
     gg.check_status()
 
 
+def test_what_another_stream_reports_is_seen():
+    """The check waits for every stream of the device, not for the current one alone."""
+    bad, stream = torch.tensor([[9]], device="cuda"), torch.cuda.Stream()
+    plan_tokens(torch.tensor([[0]], device="cuda"), 4)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(200_000_000)
+        plan_tokens(bad, 4)
+    with pytest.raises(RuntimeError, match="expert id"):
+        gg.check_status()
+    gg.check_status()
+
+
 def test_captured_and_replayed():
     torch.manual_seed(0)
     idx = _routing(50, 8, 4, "some masked").cuda()
