@@ -9,10 +9,13 @@ dispatch/combine; these ops are the expert compute that sits between them on the
 
 from __future__ import annotations
 
+import threading
+
 import torch
 
 PLAIN, SWIGLU = 0, 1
 _status: dict[int, torch.Tensor] = {}
+_status_lock = threading.Lock()
 
 
 def _ext():
@@ -26,7 +29,12 @@ def status_tensor(device) -> torch.Tensor:
     if index is None:
         index = torch.cuda.current_device()
     if index not in _status:
-        _status[index] = torch.zeros(4, dtype=torch.int32, device=torch.device("cuda", index))
+        with _status_lock:
+            if index not in _status:
+                made = torch.zeros(4, dtype=torch.int32, device=torch.device("cuda", index))
+                if not torch.cuda.is_current_stream_capturing():
+                    torch.cuda.current_stream(index).synchronize()  # kernels on other streams write to it as well, from the next call on
+                _status[index] = made
     return _status[index]
 
 

@@ -210,6 +210,20 @@ def test_what_another_stream_reports_is_seen():
     gg.check_status()
 
 
+def test_the_first_call_of_a_device_does_not_clear_what_the_next_one_reports(monkeypatch):
+    monkeypatch.setattr(gg, "_status", {})
+    good, bad, streams = torch.tensor([[0]], device="cuda"), torch.tensor([[9]], device="cuda"), [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(streams[0]):
+        torch.cuda._sleep(200_000_000)
+        plan_tokens(good, 4)
+    with torch.cuda.stream(streams[1]):
+        plan_tokens(bad, 4)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="expert id"):
+        gg.check_status()
+
+
 def test_captured_and_replayed():
     torch.manual_seed(0)
     idx = _routing(50, 8, 4, "some masked").cuda()
