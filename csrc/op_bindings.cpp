@@ -549,14 +549,14 @@ struct UnsortNode : torch::autograd::Function<UnsortNode> {
 void bind_ops(pybind11::module_& m) {
     namespace py = pybind11;
     m.def("rms_norm", &rms_norm, py::arg("x"), py::arg("weight"), py::arg("residual"), py::arg("eps"), py::arg("quantize"), py::arg("keep"), py::arg("save"));
-    m.def("rms_norm_node", [](const at::Tensor& x, const at::Tensor& weight, const OptTensor& residual, double eps, bool quantize) -> std::vector<OptTensor> {
+    m.def("rms_norm_node", [](const at::Tensor& x, const at::Tensor& weight, const OptTensor& residual, double eps, bool quantize, bool save) -> std::vector<OptTensor> {
         const auto out = NormNode::apply(x, weight, residual, eps, quantize);
         size_t at = 1;
         std::vector<OptTensor> named(5);
         named[0] = out[0];
         if (residual.has_value()) named[3] = out[at++];
         if (quantize) named[1] = out[at], named[2] = out[at + 1];
-        named[4] = out.back();
+        if (save) named[4] = out.back();
         return named;
     });
     m.def("sort_tokens_node", [](const at::Tensor& x, const at::Tensor& slots, const at::Tensor& slot_map, bool zero_padding) {

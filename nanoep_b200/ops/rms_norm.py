@@ -39,7 +39,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, *, residual: torch.Tensor | 
         if not keep:
             raise ValueError("gradients pass through y: keep=True")
         refuse_captured_gradients("rms_norm", "rms_norm_grad")
-        return NormResult(*_ext().rms_norm_node(x, weight, residual, float(eps), bool(quantize)))
+        return NormResult(*_ext().rms_norm_node(x, weight, residual, float(eps), bool(quantize), bool(save)))
     return NormResult(*_ext().rms_norm(x, weight, residual, float(eps), bool(quantize), bool(keep), bool(save)))
 
 

@@ -233,6 +233,17 @@ def test_gradient_of_the_stream_alone_and_without_rows():
     assert got.q.shape == (0, 64) and got.scales.shape == (0, 1) and dx.shape == (0, 64) and not dw.any()
 
 
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("quantize", [False, True])
+@pytest.mark.parametrize("save", [False, True])
+@pytest.mark.parametrize("with_residual", [False, True])
+def test_what_was_not_asked_for_is_none(grad, quantize, save, with_residual):
+    x, r, w = torch.randn(2, 64, device="cuda"), torch.randn(2, 64, device="cuda"), torch.ones(64, device="cuda", requires_grad=grad)
+    got = rms_norm(x, w, residual=r if with_residual else None, quantize=quantize, save=save)
+    assert [t is not None for t in got] == [True, quantize, quantize, with_residual, save]
+    assert got.y.requires_grad == grad and (got.rstd is None or not got.rstd.requires_grad)
+
+
 def test_differentiable_once():
     x = torch.randn(2, 64, device="cuda", requires_grad=True)
     w = torch.ones(64, device="cuda", requires_grad=True)
