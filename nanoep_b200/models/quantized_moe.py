@@ -41,8 +41,8 @@ class QuantizedMoE:
 
     def forward(self, x: torch.Tensor, topk_idx: torch.Tensor | None = None, topk_weights: torch.Tensor | None = None, *,
                 residual: torch.Tensor | None = None, router=None, bias: torch.Tensor | None = None):
-        """``x`` ``[T, H]``; ``topk_idx`` int64 ``[T, K]`` (-1 = masked) and ``topk_weights`` fp32 ``[T, K]``, or ``router``, which gives both from the normed rows.
-        Returns ``out`` bf16 ``[T, H]`` (plus ``bias`` ``[T, H]``, a shared expert's output), or ``(out, x + residual)`` where a ``residual`` is given."""
+        """``x`` ``[T, H]`` bf16, fp16 or fp32 (with a norm: ``norm_weight`` of that type or fp32); ``topk_idx`` int64 ``[T, K]`` (-1 = masked) and ``topk_weights`` fp32 ``[T, K]``, or ``router``, which gives both from the normed rows.
+        Returns ``out`` bf16 ``[T, H]`` (plus ``bias`` bf16 ``[T, H]``, a shared expert's output), or ``(out, x + residual)`` where a ``residual`` is given."""
         refuse_gradients("QuantizedMoE", x, topk_weights, residual, bias, self.norm_weight, self.w13, self.w13_scales, self.w2, self.w2_scales)
         stream = None
         if self.norm_weight is not None:

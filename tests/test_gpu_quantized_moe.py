@@ -92,6 +92,29 @@ def test_layer(tokens, hidden, inner, experts, topk, norm):
     gg.check_status()
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("norm", [True, False])
+def test_rows_of_other_types(dtype, norm):
+    """Rows in fp16 or fp32: the result stays bf16, and so does what is added to it."""
+    layer = _layer(8, 512, 256, norm)
+    if norm:
+        layer.norm_weight = layer.norm_weight.to(dtype)
+    x, idx, gate = _batch(70, 512, 8, 2)
+    x, bias = x.to(dtype), torch.randn(70, 512, device="cuda").to(torch.bfloat16)
+    want, _ = _reference(layer, x, idx, gate, None)
+    out = layer(x, idx, gate, bias=bias)
+    assert out.dtype == torch.bfloat16
+    _near(out, want + bias.double())
+    if norm:
+        residual = torch.randn(70, 512, device="cuda").to(dtype)
+        out, stream = layer(x, idx, gate, residual=residual)
+        want, h = _reference(layer, x, idx, gate, residual)
+        _near(out, want)
+        assert stream.dtype == dtype and torch.equal(stream, h)
+    with pytest.raises(RuntimeError, match="bias"):
+        layer(x, idx, gate, bias=bias.to(dtype))
+
+
 def test_between_dispatch_and_combine(monkeypatch):
     """The 8-bit products on a dispatch's rows: aligned ranges, counts that leave padding rows out, gate weights in the product, and a combine behind them."""
     monkeypatch.setenv("LOCAL_RANK", "0")

@@ -68,6 +68,43 @@ def test_forward(tokens, hidden, dtype, wide, with_residual):
     assert torch.equal(only.q.view(torch.uint8), got.q.view(torch.uint8)) and torch.equal(only.scales, got.scales)
 
 
+@pytest.mark.parametrize("tokens,hidden", [(5000, 520), (1000, 7168), (700, 16384)])
+@pytest.mark.parametrize("dtype,wide", [(torch.bfloat16, False), (torch.bfloat16, True), (torch.float16, False), (torch.float32, False)])
+@pytest.mark.parametrize("with_residual", [False, True])
+def test_several_rows_a_block(tokens, hidden, dtype, wide, with_residual):
+    """More rows than twice the blocks of a launch: the next row's loads under the row before, sums by turns, in every width of a thread."""
+    units = hidden // 8
+    per = 1 if units <= 512 else 2 if units <= 1024 else 4
+    threads = -(-(-(-units // per)) // 32) * 32
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert tokens > 2 * sms * max(1, min(16, (1536 if per == 1 else 1024) // threads)) and per == (1, 2, 4)[(520, 7168, 16384).index(hidden)]
+    gen = torch.Generator(device="cuda").manual_seed(hidden)
+    x = torch.randn(tokens, hidden, generator=gen, device="cuda").to(dtype) * torch.exp2(torch.randint(-3, 4, (tokens, 1), generator=gen, device="cuda")).to(dtype)
+    residual = torch.randn(tokens, hidden, generator=gen, device="cuda").to(dtype) if with_residual else None
+    weight = (torch.randn(hidden, generator=gen, device="cuda") * 0.3 + 1).to(torch.float32 if wide else dtype)
+    got = rms_norm(x, weight, residual=residual, eps=1e-5, quantize=True, save=True)
+    for first in range(0, tokens, 1000):
+        part = slice(first, first + 1000)
+        h, v, rstd = _reference(x[part], weight, residual[part] if with_residual else None, 1e-5)
+        assert not with_residual or torch.equal(got.residual[part], h)
+        torch.testing.assert_close(got.rstd[part].double(), rstd[:, 0], rtol=EPS32, atol=0)
+        torch.testing.assert_close(got.y[part].double(), v * rstd, rtol=_half_step(dtype) + 2 * EPS32, atol=SMALLEST[dtype])
+        _check_quantized(got.q[part], got.scales[part], v, rstd, exact=False)
+
+
+def test_gradients_of_both_inputs_are_tensors_of_their_own():
+    """x and the residual have the same gradient; a step that changes one in place leaves the other."""
+    x, r = (torch.randn(4, 64, device="cuda", requires_grad=True) for _ in range(2))
+    got = rms_norm(x, torch.ones(64, device="cuda"), residual=r)
+    g = torch.randn(4, 64, device="cuda")
+    torch.autograd.backward((got.y, got.residual), (g, g))
+    assert torch.equal(x.grad, r.grad) and x.grad.data_ptr() != r.grad.data_ptr()
+    x.grad, r.grad = None, None
+    rms_norm(x, torch.ones(64, device="cuda"), residual=r).residual.backward(g)
+    x.grad.zero_()
+    assert bool(r.grad.any()) and bool(g.any())
+
+
 def test_rows_that_do_not_start_on_16_bytes():
     x = torch.randn(4, 256, device="cuda").to(torch.bfloat16)
     shifted = torch.empty(4 * 256 + 1, device="cuda", dtype=torch.bfloat16)[1:].view(4, 256)
