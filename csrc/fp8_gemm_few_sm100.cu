@@ -14,7 +14,8 @@
 //
 // What bounds it: the weights' way from memory (32 experts of 7168 x 2048, up, us: 1 row each 150, 16 rows 154, 32 rows 159 = 5.9 TB/s, where a
 // copy runs at 6.5; rows as M 171, 172, 176), and for one matrix that of few SMs, 78 GB/s each, behind about 8 us of launch, setup and
-// exchange: 7168 x 4096 with one row 28.5 us in one CTA a tile, 18.5 in two, 14.1 in four, 12.4 in four on tiles of 128 weight rows.
+// exchange: 7168 x 4096 with one row, calls on eight such matrices by turns in a graph, 25.1 us in one CTA a tile, 16.6 in two, 13.0 in four, 12.7 in
+// four on tiles of 128 weight rows.
 //
 // Tried: 16 columns of both accumulators per wait instead of 8: 64 rows each 193 -> 200 us; the state of the next barriers asked for under the
 // MMAs: within the spread; 128 rows as N: 312 us at 128 rows each (the columns' scales), rows as M 188.
@@ -216,9 +217,9 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_few_kernel(const __grid_
                     for (int i = 0; i < kAcc; ++i)
                         tma_load_3d(dst + i * kLanesBytes, &maps.weights, kb * 128, kSwiGLU ? t.nt * kLanes : (kAcc * t.nt + i) * kLanes,
                                     kSwiGLU ? 2 * t.expert + i : t.expert, &sh.full[stage]);
-                    int at = 0;  // boxes of 128, 64, 32 and 16 rows make up any multiple of 16
+                    int at = 0;  // boxes of 64, 32 and 16 rows make up any multiple of 16 that a tile has
 #pragma unroll
-                    for (int b = 0; b < 4; ++b) {
+                    for (int b = kTileRows <= 32 ? 2 : 1; b < 4; ++b) {
                         const int box = 128 >> b;
                         if (n & box) {
                             tma_load_2d(dst + P::kWeightBytes + at * 128, &maps.rows[b], kb * 128, t.row0 + at, &sh.full[stage]);
@@ -407,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_few_kernel(const __grid_
                     const int64_t row = int64_t(t.row0) + in_tile;
                     if (kSwiGLU) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) v[0][j] = __fdividef(v[0][j], 1.f + __expf(-v[0][j])) * v[kAcc - 1][j];
+                        for (int j = 0; j < 4; ++j) v[0][j] = swiglu(v[0][j], v[kAcc - 1][j]);
                     } else if (args.row_scale != nullptr) {
                         const float f = args.row_scale[row];
 #pragma unroll

@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_gemm_kernel(const __grid_cons
             const int n0 = kSwiGLU ? t.nt * 128 + group * 64 : t.nt * kTileCols + group * 128;
             if (kSwiGLU) {
 #pragma unroll
-                for (int j = 0; j < 64; ++j) acc[j] = __fdividef(acc[j], 1.f + __expf(-acc[j])) * acc[64 + j];
+                for (int j = 0; j < 64; ++j) acc[j] = swiglu(acc[j], acc[64 + j]);
             } else if (args.row_scale != nullptr) {
 #pragma unroll
                 for (int j = 0; j < 128; ++j) acc[j] *= out_scale;

@@ -79,6 +79,10 @@ __device__ __forceinline__ void mma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint6
                  : "memory");
 }
 
+// silu(gate) * up.  The quotient is the fast one, a choice: within 2 units in the last place, and 0 for gates below -87.3 (1 + exp(-gate) is beyond 2^126 there),
+// whose silu is below 2^-119 in size.  A rounded quotient, as the 16-bit kernels' epilogue has: 4096 tokens, 32 experts, up 1350 -> 1490 us.
+__device__ __forceinline__ float swiglu(float gate, float up) { return __fdividef(gate, 1.f + __expf(-gate)) * up; }
+
 __device__ __forceinline__ uint64_t pair_of(float f) {
     uint64_t p;
     asm("mov.b64 %0, {%1, %1};" : "=l"(p) : "r"(__float_as_uint(f)));

@@ -349,9 +349,9 @@ void check_i64(const OptTensor& t, const at::Tensor& a, int64_t entries, const c
 // The choice is the shortest of the times that these kernels have taken, whole passes over the tiles at a time.  us a block of 128 columns: rows
 // as M 0.62 on a few SMs and 0.69 on all; 32 rows as N 0.43 alone, 0.70 where all SMs stream weights from memory, 0.45 where L2 has
 // them; 64 rows 0.61 and 0.86.  Behind a tile's last block: 2.7, and 2.5 + 0.3 a CTA for the exchange.  32 experts of 7168 x 2048, up, us for 32
-// rows as N, 64, and rows as M: 32 rows an expert 157, 166, 172; 64 rows 199, 192, 174.  One matrix of 7168 x 4096: one row 14 over four
-// CTAs, 27 in one, 35; 128 rows 27, 21, 38.  Tiles of one block of output columns instead of two (0.62 of a block's time each): one row 12.4
-// instead of 14.1, 64 rows 17.9 instead of 16.4.
+// rows as N, 64, and rows as M: 32 rows an expert 157, 166, 172; 64 rows 199, 192, 174.  One matrix of 7168 x 4096, calls on eight such matrices by turns in a graph: one row
+// 13.0 over four CTAs, 25.1 in one, 36.4; 128 rows, four CTAs, 23.1, 19.0, 41.0.  Tiles of one block of output columns instead of two (0.62 of a block's time each): one
+// row 12.7 instead of 13.0, 64 rows (as 32s) 20.4 instead of 15.1.
 struct Fp8Choice {
     int64_t tile, ctas, units, n_tiles;
 };
