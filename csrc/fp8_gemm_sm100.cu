@@ -17,7 +17,7 @@
 // and the MMAs, which read 48 KB of the same shared memory, and the rest that an epilogue warp gets through 128 columns in 0.6 us:
 // under this traffic a load from shared memory or a look at a barrier takes 200 to 300 cycles.  Hence: no fence where a value read says
 // enough, scales and the next block's state asked for a block ahead, the tile's description left by the warp that loads the scales.
-// In a long run the power limit (1000 W, 1.6 GHz): 32 x (1024 +- 32) rows up 1325 us = 1.45 PFLOP/s of real rows, down 650 us.
+// In a long run the power limit (1000 W, 1.6 GHz): 32 x (1024 +- 32) rows up 1340 us = 1.44 PFLOP/s of real rows, down 650 us.
 //
 // Tried: pairs of CTAs (cta_group::2, 256 rows, two thirds of the operand traffic): 0.69 us a block as well, with a signal between the CTAs in every
 // block; at 128 rows an expert half of a pair is idle (up 257 us instead of 188).  Two columns per instruction (fma.rn.f32x2): no faster, and
