@@ -61,8 +61,8 @@ def grouped_gemm_fp8(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w
     expert_offsets: int64 ``[E + 1]``, not falling, from 0 to at most ``rows``, of any alignment; rows behind the last are not written.
     ``expert_counts`` (int64 ``[E]``): only so many rows of each range exist, the others are neither read nor written.
     ``row_scale`` (fp32 ``[rows]``, not with ``swiglu``) multiplies each output row before it is rounded.
-    ``max_expert_rows`` (0 = unknown): no expert holds more rows.  The tile is chosen for so many rows, or for the average of the ranges where that is less and
-    more than 32; it matters where ranges are padded, as behind a dispatch.  The result depends on it only in its rounding.
+    ``max_expert_rows`` (0 = unknown): no expert holds more rows.  The tile is chosen for so many rows where they are at most 32, else for the average of the
+    ranges where that is less; it matters where ranges are padded, as behind a dispatch.  The result depends on it only in its rounding.
     """
     refuse_gradients("grouped_gemm_fp8", a, a_scales, w, w_scales, row_scale)
     if w.dim() == 2:
